@@ -21,8 +21,8 @@ ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
 
 KERNEL_SOURCES = ["rmsnorm.hip", "rope.hip", "swiglu.hip", "cross_entropy.hip", "fp8_cast.hip",
                   "attention.hip", "mfma_probe.hip", "gemm_bench.hip",
-                  "grouped_gemm.hip"]
-HEADERS = ["common.h"]
+                  "grouped_gemm.hip", "vocab.hip"]
+HEADERS = ["common.h", "vocab.h"]
 
 
 def _newest_mtime(paths):

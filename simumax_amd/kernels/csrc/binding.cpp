@@ -2,8 +2,12 @@
 // Compiled directly with hipcc (no hipify pass) by kernels/build.py.
 #include <torch/extension.h>
 
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
+
+#include "vocab.h"
 
 #define CHECK_IN(t)                                                     \
     TORCH_CHECK((t).is_cuda(), #t " must be on GPU");                   \
@@ -276,6 +280,228 @@ void fp8_cast_t(torch::Tensor x, torch::Tensor out, torch::Tensor out_t,
                       e5m2 ? 1 : 0, (float)fmax, cur_stream());
 }
 
+// ---- operators over the rows of logits (see vocab.hip) ----
+extern "C" {
+int vocab_segment(int);
+void logprobs_fwd_launch(const VocabRows *, const VocabLogprobs *, int,
+                         hipStream_t);
+void distill_fwd_launch(const VocabRows *, const VocabDistill *, int,
+                        hipStream_t);
+void vocab_grad_launch(const VocabRows *, const VocabGrad *, int, void *, int,
+                       hipStream_t);
+}
+
+static int vocab_dtype(const torch::Tensor &t) {
+    switch (t.scalar_type()) {
+        case torch::kBFloat16: return VOCAB_BF16;
+        case torch::kFloat16: return VOCAB_FP16;
+        case torch::kFloat32: return VOCAB_FP32;
+        default: TORCH_CHECK(false, "logits must be bf16, fp16 or fp32");
+    }
+}
+
+// the rows of [..., V] logits as at most two strided dimensions; false if
+// their strides need more than that
+static bool vocab_rows(const torch::Tensor &x, VocabRows *g) {
+    TORCH_CHECK(x.is_cuda(), "logits must be on GPU");
+    TORCH_CHECK(x.dim() >= 1, "logits must be [..., V]");
+    const int64_t V = x.size(-1);
+    TORCH_CHECK(V >= 1 && V < (1ll << 31), "vocabulary of ", V, " tokens");
+    if (V > 1 && x.stride(-1) != 1) return false;
+    int64_t rows = 1;
+    std::vector<std::pair<int64_t, int64_t>> dims;  // (size, stride), merged
+    for (int i = 0; i + 1 < x.dim(); ++i) {
+        rows *= x.size(i);
+        if (x.size(i) == 1) continue;
+        if (!dims.empty() && dims.back().second == x.stride(i) * x.size(i)) {
+            dims.back().first *= x.size(i);
+            dims.back().second = x.stride(i);
+        } else {
+            dims.emplace_back(x.size(i), x.stride(i));
+        }
+    }
+    TORCH_CHECK(rows < (1ll << 31), rows, " rows of logits");
+    if (dims.size() > 2) return false;
+    while (dims.size() < 2) dims.insert(dims.begin(), {1, 0});
+    g->base = x.data_ptr();
+    g->V = V;
+    g->stride_o = dims[0].second;
+    g->stride_i = dims[1].second;
+    g->rows = (int)rows;
+    g->inner = (int)std::max<int64_t>(dims[1].first, 1);
+    const int seg = vocab_segment(vocab_dtype(x));
+    g->nseg = (int)((V + seg - 1) / seg);
+    return true;
+}
+
+static VocabRows vocab_rows_or_copy(torch::Tensor &x) {
+    VocabRows g;
+    if (!vocab_rows(x, &g)) {
+        x = x.contiguous();
+        TORCH_CHECK(vocab_rows(x, &g));
+    }
+    return g;
+}
+
+#define CHECK_ROWS(t, type, n)                                           \
+    CHECK_IN(t);                                                         \
+    TORCH_CHECK((t).device() == logits.device(),                         \
+                #t " must be on the device of the logits");              \
+    TORCH_CHECK((t).scalar_type() == (type), #t " has the wrong dtype"); \
+    TORCH_CHECK((t).numel() == (int64_t)(n), #t " has the wrong size")
+
+static std::vector<int64_t> lead_sizes(const torch::Tensor &x) {
+    auto s = x.sizes().vec();
+    s.pop_back();
+    return s;
+}
+
+// -> logprobs, entropy, top_logprobs, top_ids, stat
+std::vector<torch::Tensor> token_logprobs_fwd(
+    torch::Tensor logits, c10::optional<torch::Tensor> tokens, int64_t topk,
+    double temperature, int64_t ignore_index) {
+    c10::OptionalDeviceGuard guard(logits.device());
+    VocabRows g = vocab_rows_or_copy(logits);
+    TORCH_CHECK(topk >= 0 && topk <= VOCAB_MAX_K && topk <= g.V, "topk");
+    TORCH_CHECK(temperature > 0, "temperature");
+    if (tokens) {
+        CHECK_ROWS(*tokens, torch::kInt64, g.rows);
+    }
+    const auto f32 = logits.options().dtype(torch::kFloat32);
+    const auto lead = lead_sizes(logits);
+    auto top_shape = lead;
+    top_shape.push_back(topk);
+    auto logprobs = torch::empty(tokens ? lead : std::vector<int64_t>{0}, f32);
+    auto entropy = torch::empty(lead, f32);
+    auto top_lp = torch::empty(top_shape, f32);
+    auto top_ids = torch::empty(top_shape, f32.dtype(torch::kInt64));
+    auto stat = torch::empty({g.rows, 4}, f32);
+    if (g.rows > 0) {
+        auto part = torch::empty({g.rows, g.nseg, 4}, f32);
+        VocabLogprobs a;
+        a.tokens = tokens ? tokens->data_ptr<int64_t>() : nullptr;
+        a.ignore = ignore_index;
+        a.K = (int)topk;
+        a.temperature = temperature;
+        a.part = part.data_ptr<float>();
+        a.logprobs = logprobs.data_ptr<float>();
+        a.entropy = entropy.data_ptr<float>();
+        a.top_lp = top_lp.data_ptr<float>();
+        a.top_ids = top_ids.data_ptr<int64_t>();
+        a.stat = stat.data_ptr<float>();
+        logprobs_fwd_launch(&g, &a, vocab_dtype(logits), cur_stream());
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+    }
+    return {logprobs, entropy, top_lp, top_ids, stat};
+}
+
+torch::Tensor token_logprobs_bwd(
+    torch::Tensor logits, c10::optional<torch::Tensor> tokens,
+    torch::Tensor top_ids, torch::Tensor stat,
+    c10::optional<torch::Tensor> d_logprobs,
+    c10::optional<torch::Tensor> d_entropy, c10::optional<torch::Tensor> d_top,
+    double temperature, int64_t ignore_index) {
+    c10::OptionalDeviceGuard guard(logits.device());
+    VocabRows g = vocab_rows_or_copy(logits);
+    const int64_t K = top_ids.size(-1);
+    TORCH_CHECK(K <= VOCAB_MAX_K, "topk");
+    CHECK_ROWS(stat, torch::kFloat32, g.rows * 4ll);
+    CHECK_ROWS(top_ids, torch::kInt64, g.rows * K);
+    VocabGrad a = {};
+    if (tokens) {
+        CHECK_ROWS(*tokens, torch::kInt64, g.rows);
+        a.tokens = tokens->data_ptr<int64_t>();
+    }
+    if (d_logprobs) {
+        CHECK_ROWS(*d_logprobs, torch::kFloat32, g.rows);
+        a.d_row = d_logprobs->data_ptr<float>();
+    }
+    if (d_entropy) {
+        CHECK_ROWS(*d_entropy, torch::kFloat32, g.rows);
+        a.d_entropy = d_entropy->data_ptr<float>();
+    }
+    if (d_top) {
+        CHECK_ROWS(*d_top, torch::kFloat32, g.rows * K);
+        a.d_top = d_top->data_ptr<float>();
+    }
+    a.stat = (const float4 *)stat.data_ptr<float>();
+    a.c = (float)(1.4426950408889634 / temperature);
+    a.inv_t = (float)(1. / temperature);
+    a.K = (int)K;
+    a.ids = top_ids.data_ptr<int64_t>();
+    a.ignore = ignore_index;
+    auto out = torch::empty(logits.sizes(), logits.options());
+    if (g.rows > 0) {
+        vocab_grad_launch(&g, &a, 0, out.data_ptr(), vocab_dtype(logits),
+                          cur_stream());
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+    }
+    return out;
+}
+
+// -> loss, q, stat
+std::vector<torch::Tensor> topk_distillation_fwd(torch::Tensor logits,
+                                                 torch::Tensor teacher_logprobs,
+                                                 torch::Tensor teacher_ids,
+                                                 double temperature,
+                                                 bool bucket) {
+    c10::OptionalDeviceGuard guard(logits.device());
+    VocabRows g = vocab_rows_or_copy(logits);
+    const int64_t K = teacher_ids.size(-1);
+    TORCH_CHECK(K >= 1 && K <= VOCAB_MAX_K, "entries per row");
+    TORCH_CHECK(temperature > 0, "temperature");
+    CHECK_ROWS(teacher_ids, torch::kInt64, g.rows * K);
+    CHECK_ROWS(teacher_logprobs, torch::kFloat32, g.rows * K);
+    const auto f32 = logits.options().dtype(torch::kFloat32);
+    auto loss = torch::empty(lead_sizes(logits), f32);
+    auto q = torch::empty({g.rows, K}, f32);
+    auto stat = torch::empty({g.rows, 4}, f32);
+    if (g.rows > 0) {
+        auto part = torch::empty({g.rows, g.nseg, 4}, f32);
+        VocabDistill a;
+        a.teacher_lp = teacher_logprobs.data_ptr<float>();
+        a.ids = teacher_ids.data_ptr<int64_t>();
+        a.K = (int)K;
+        a.bucket = bucket ? 1 : 0;
+        a.temperature = temperature;
+        a.part = part.data_ptr<float>();
+        a.loss = loss.data_ptr<float>();
+        a.q = q.data_ptr<float>();
+        a.stat = stat.data_ptr<float>();
+        distill_fwd_launch(&g, &a, vocab_dtype(logits), cur_stream());
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+    }
+    return {loss, q, stat};
+}
+
+torch::Tensor topk_distillation_bwd(torch::Tensor dloss, torch::Tensor logits,
+                                    torch::Tensor teacher_ids, torch::Tensor q,
+                                    torch::Tensor stat, double temperature) {
+    c10::OptionalDeviceGuard guard(logits.device());
+    VocabRows g = vocab_rows_or_copy(logits);
+    const int64_t K = teacher_ids.size(-1);
+    TORCH_CHECK(K >= 1 && K <= VOCAB_MAX_K, "entries per row");
+    CHECK_ROWS(dloss, torch::kFloat32, g.rows);
+    CHECK_ROWS(teacher_ids, torch::kInt64, g.rows * K);
+    CHECK_ROWS(q, torch::kFloat32, g.rows * K);
+    CHECK_ROWS(stat, torch::kFloat32, g.rows * 4ll);
+    VocabGrad a = {};
+    a.stat = (const float4 *)stat.data_ptr<float>();
+    a.c = (float)(1.4426950408889634 / temperature);
+    a.inv_t = (float)(1. / temperature);
+    a.K = (int)K;
+    a.d_row = dloss.data_ptr<float>();
+    a.q = q.data_ptr<float>();
+    a.ids = teacher_ids.data_ptr<int64_t>();
+    auto out = torch::empty(logits.sizes(), logits.options());
+    if (g.rows > 0) {
+        vocab_grad_launch(&g, &a, 1, out.data_ptr(), vocab_dtype(logits),
+                          cur_stream());
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+    }
+    return out;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("fp8_cast", &fp8_cast,
           "fused bf16->fp8 cast + running amax (delayed scaling)");
@@ -299,4 +525,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "grouped expert GEMM dgrad: [E,M,N]x[E,N,K] -> [E,M,K] (MFMA)");
     m.def("grouped_wgrad", &grouped_wgrad,
           "grouped expert wgrad: fp32 G[E,N,K] += dout^T @ x (MFMA)");
+    m.def("token_logprobs_fwd", &token_logprobs_fwd,
+          "log probabilities, entropy, top alternatives of logits (gfx950)");
+    m.def("token_logprobs_bwd", &token_logprobs_bwd,
+          "gradient of token_logprobs_fwd (gfx950)");
+    m.def("topk_distillation_fwd", &topk_distillation_fwd,
+          "divergence from a teacher's top log probabilities (gfx950)");
+    m.def("topk_distillation_bwd", &topk_distillation_bwd,
+          "gradient of topk_distillation_fwd (gfx950)");
 }

@@ -1,0 +1,49 @@
+// Arguments that the vocabulary kernels (vocab.hip) share with their torch
+// binding.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#define VOCAB_MAX_K 256  // top alternatives, or a teacher's entries, per row
+
+enum { VOCAB_BF16 = 0, VOCAB_FP16 = 1, VOCAB_FP32 = 2 };
+
+// rows of V logits, contiguous within a row; row r = o * inner + i starts at
+// base + o * stride_o + i * stride_i (in elements)
+struct VocabRows {
+    const void *base;
+    long V, stride_o, stride_i;
+    int rows, inner, nseg;  // nseg: stretches per row
+};
+
+struct VocabLogprobs {
+    const long *tokens;  // [rows] or null
+    long ignore;
+    int K;
+    double temperature;
+    float *part;  // [rows, nseg, 4] workspace
+    float *logprobs, *entropy, *top_lp;
+    long *top_ids;
+    float *stat;  // [rows, 4]
+};
+
+struct VocabDistill {
+    const float *teacher_lp;  // [rows, K]
+    const long *ids;          // [rows, K]
+    int K, bucket;
+    double temperature;
+    float *part, *loss, *q, *stat;
+};
+
+struct VocabGrad {
+    const float4 *stat;
+    float c, inv_t;
+    int K;
+    const float *d_row;      // of the log probabilities, or of the loss
+    const float *d_entropy;  // null where none
+    const float *d_top;      // [rows, K], null where none
+    const float *q;          // [rows, K], the teacher's weights
+    const long *ids;         // [rows, K]
+    const long *tokens;      // [rows] or null
+    long ignore;
+};

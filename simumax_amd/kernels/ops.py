@@ -399,3 +399,10 @@ def flash_attention(q, k, v, causal=True):
     """q [B,S,Hq,D], k/v [B,S,Hkv,D] (GQA) -> [B,S,Hq,D]."""
     return _FlashAttnFn.apply(q.contiguous(), k.contiguous(), v.contiguous(),
                               causal)
+
+
+# --------------------------------------------------------------------------
+# Post-training operators on the logits (see vocab.py)
+# --------------------------------------------------------------------------
+from .vocab import (TokenLogprobs, token_logprobs,  # noqa: E402,F401
+                    topk_distillation)
