@@ -283,6 +283,7 @@ void fp8_cast_t(torch::Tensor x, torch::Tensor out, torch::Tensor out_t,
 // ---- operators over the rows of logits (see vocab.hip) ----
 extern "C" {
 int vocab_segment(int);
+int vocab_group(void);
 void logprobs_fwd_launch(const VocabRows *, const VocabLogprobs *, int,
                          hipStream_t);
 void distill_fwd_launch(const VocabRows *, const VocabDistill *, int,
@@ -363,6 +364,8 @@ std::vector<torch::Tensor> token_logprobs_fwd(
     c10::OptionalDeviceGuard guard(logits.device());
     VocabRows g = vocab_rows_or_copy(logits);
     TORCH_CHECK(topk >= 0 && topk <= VOCAB_MAX_K && topk <= g.V, "topk");
+    TORCH_CHECK(topk == 0 || g.V <= VOCAB_MAX_TOP_V,
+                "top alternatives of a vocabulary above ", VOCAB_MAX_TOP_V);
     TORCH_CHECK(temperature > 0, "temperature");
     if (tokens) {
         CHECK_ROWS(*tokens, torch::kInt64, g.rows);
@@ -378,7 +381,13 @@ std::vector<torch::Tensor> token_logprobs_fwd(
     auto stat = torch::empty({g.rows, 4}, f32);
     if (g.rows > 0) {
         auto part = torch::empty({g.rows, g.nseg, 4}, f32);
+        const int dt = vocab_dtype(logits);
+        torch::Tensor gmax;
+        if (topk > 0)
+            gmax = torch::empty({g.rows, g.nseg,
+                                 vocab_segment(dt) / vocab_group()}, f32);
         VocabLogprobs a;
+        a.gmax = topk > 0 ? gmax.data_ptr<float>() : nullptr;
         a.tokens = tokens ? tokens->data_ptr<int64_t>() : nullptr;
         a.ignore = ignore_index;
         a.K = (int)topk;
@@ -389,7 +398,7 @@ std::vector<torch::Tensor> token_logprobs_fwd(
         a.top_lp = top_lp.data_ptr<float>();
         a.top_ids = top_ids.data_ptr<int64_t>();
         a.stat = stat.data_ptr<float>();
-        logprobs_fwd_launch(&g, &a, vocab_dtype(logits), cur_stream());
+        logprobs_fwd_launch(&g, &a, dt, cur_stream());
         C10_HIP_KERNEL_LAUNCH_CHECK();
     }
     return {logprobs, entropy, top_lp, top_ids, stat};

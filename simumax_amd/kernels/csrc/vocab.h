@@ -6,6 +6,8 @@
 
 #define VOCAB_MAX_K 256  // top alternatives, or a teacher's entries, per row
 
+#define VOCAB_MAX_TOP_V 524288  // vocabulary, where top alternatives are asked
+
 enum { VOCAB_BF16 = 0, VOCAB_FP16 = 1, VOCAB_FP32 = 2 };
 
 // rows of V logits, contiguous within a row; row r = o * inner + i starts at
@@ -22,6 +24,7 @@ struct VocabLogprobs {
     int K;
     double temperature;
     float *part;  // [rows, nseg, 4] workspace
+    float *gmax;  // [rows, nseg, segment / group] workspace, where K > 0
     float *logprobs, *entropy, *top_lp;
     long *top_ids;
     float *stat;  // [rows, 4]

@@ -21,12 +21,16 @@
 // No floating-point atomics: the same input gives the same bits.
 #include <hip/hip_fp16.h>
 
+#include <type_traits>
+
 #include "common.h"
 #include "vocab.h"
 
 #define BLOCK 256
 #define WAVES (BLOCK / WAVE)
-#define NVEC 8  // 16-byte vectors per lane and stretch
+#define NVEC 8    // 16-byte vectors per lane and stretch
+#define GROUP 64  // tokens per maximum kept for the top alternatives
+#define CAP 512   // candidates for them that are ranked at once
 
 typedef unsigned int u32;
 typedef unsigned long long u64;
@@ -160,15 +164,33 @@ DEV double block_sum_d(double v, double *lds) {
     return r;
 }
 
+// maximum over aligned groups of LPG = 8 or 16 lanes, in every lane
+template <int CTRL> DEV float max_dpp(float v) {
+    const int o = __builtin_amdgcn_update_dpp(
+        __float_as_int(v), __float_as_int(v), CTRL, 0xf, 0xf, false);
+    return fmaxf(v, __int_as_float(o));
+}
+template <int LPG> DEV float group_max(float v) {
+    v = max_dpp<0xB1>(v);   // quad_perm [1, 0, 3, 2]
+    v = max_dpp<0x4E>(v);   // quad_perm [2, 3, 0, 1]
+    v = max_dpp<0x141>(v);  // row_half_mirror: the other quad of 8
+    if (LPG == 16) v = max_dpp<0x140>(v);  // row_mirror: the other 8 of 16
+    return v;
+}
+
 // ---- partials --------------------------------------------------------------
 // One wave per stretch. Writes (m, s, t, s_in): s_in is the part of the sum
 // that belongs to the teacher's entries (EXCL), and s then leaves it out:
 // the rest of the mass is summed, not got as a difference, because a
 // student that has learned leaves little of it.
-template <typename T, bool ENT, bool EXCL>
+// With GRP also the maximum of each GROUP consecutive tokens, for the search
+// of the top alternatives: 4 more operations per vector and 4 bytes per 64
+// tokens.
+template <typename T, bool ENT, bool EXCL, bool GRP>
 __global__ __launch_bounds__(BLOCK) void vocab_partials(
     VocabRows g, const long *__restrict__ tokens, long ignore,
-    const long *__restrict__ ids, int K, float c, float4 *__restrict__ part) {
+    const long *__restrict__ ids, int K, float c, float4 *__restrict__ part,
+    float *__restrict__ gmax) {
     constexpr int N = Vec<T>::N;
     constexpr int SEG = WAVE * NVEC * N;
     __shared__ u32 bits[EXCL ? WAVES : 1][EXCL ? SEG / 32 : 1];
@@ -194,11 +216,25 @@ __global__ __launch_bounds__(BLOCK) void vocab_partials(
 #pragma unroll
         for (int j = 0; j < NVEC; ++j)
             v[j] = load_vec(row, lo + (long)(j * WAVE + lane) * N, g.V);
-        float m = -INFINITY;
+        float m = -INFINITY, gm = -INFINITY;
+        constexpr int LPG = GROUP / N;  // lanes per group: 8 or 16
 #pragma unroll
-        for (int j = 0; j < NVEC; ++j)
+        for (int j = 0; j < NVEC; ++j) {
+            float vm = v[j].get(0);
 #pragma unroll
-            for (int i = 0; i < N; ++i) m = fmaxf(m, v[j].get(i));
+            for (int i = 1; i < N; ++i) vm = fmaxf(vm, v[j].get(i));
+            m = fmaxf(m, vm);
+            if (GRP) {
+                vm = group_max<LPG>(vm);
+                if (lane % LPG == j) gm = vm;
+            }
+        }
+        if (GRP) {
+            // lane (group q of a vector, j) has group j * (64 / LPG) + q
+            const int q = lane / LPG, j = lane % LPG;
+            if (j < NVEC)
+                gmax[w * (SEG / GROUP) + j * (WAVE / LPG) + q] = gm;
+        }
         m = wave_max(m);
         const float mr = m == -INFINITY ? 0.f : m, mc = mr * c;
         float s = 0.f, t = 0.f, s_in = 0.f;
@@ -264,38 +300,211 @@ DEV RowStat join_parts(const float4 *p, int nseg, float c, double *lds) {
     return st;
 }
 
-// order of 32-bit floats as whole numbers; -0 counts as 0
-DEV u32 order_of(float x) {
-    const u32 b = __float_as_uint(x + 0.f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+// ---- top alternatives ------------------------------------------------------
+// Values as whole numbers of the same order (-0 counts as 0), without the low
+// bits that the type never sets; 0 is below them all.
+template <typename T> struct Order {
+    static constexpr int LOW = sizeof(T) == 4                             ? 0
+                               : std::is_same<T, __half>::value ? 13 : 16;
+    static constexpr int BITS = 32 - LOW;
+    static DEV u32 of(float x) {
+        const u32 b = __float_as_uint(x + 0.f);
+        return (b & 0x80000000u ? ~b : b | 0x80000000u) >> LOW;
+    }
+};
+
+struct TopShared {
+    u64 key[CAP];               // (order, ~index) of the candidates
+    int group[VOCAB_MAX_K];     // groups that can hold alternatives
+    int count[2][WAVES];        // of block_count, two turns
+    int ties[32 * WAVES];
+    int n_group, n_key;
+};
+
+// number of true predicates in the workgroup, given each wave's own. `turn`
+// alternates between calls, so one barrier is enough.
+DEV int block_count(int wave_count, TopShared &sh, int &turn) {
+    if (threadIdx.x % WAVE == 0) sh.count[turn][threadIdx.x / WAVE] = wave_count;
+    __syncthreads();
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) n += sh.count[turn][w];
+    turn ^= 1;
+    return n;
 }
 
-DEV u64 block_max_u64(u64 v, u64 *lds) {
+// calls f(order, index, valid) for every token of the chosen groups; all
+// lanes take part in every call
+template <typename T, typename F>
+DEV void for_candidates(const T *row, long V, const TopShared &sh, int groups,
+                        F f) {
+    constexpr int N = Vec<T>::N, LPG = GROUP / N;
+    for (int i = 0; i < groups * LPG; i += BLOCK) {
+        const int slot = i + threadIdx.x;
+        const bool on = slot < groups * LPG;
+        const long at =
+            on ? (long)sh.group[slot / LPG] * GROUP + slot % LPG * N : V;
+        const Vec<T> v = load_vec(row, at, V);
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const u64 o = __shfl_xor(v, off, WAVE);
-        v = o > v ? o : v;
+        for (int k = 0; k < N; ++k)
+            f(Order<T>::of(v.get(k)), (u32)(at + k), at + k < V);
+    }
+}
+
+// The K largest of a row, (value down, index up), from its groups' maxima.
+// The K groups of the largest (maximum, lowest index) hold them all: each of
+// these has a token at least as good as any token of the others. The K-th
+// maximum is found by bits; tokens of those groups that reach it are the
+// candidates, hardly more than K in a row without structure; each one's rank
+// is the number of better ones. Where more than CAP reach it (groups with
+// many large tokens, or a vocabulary of few groups), a higher bound is
+// searched among the tokens themselves, and, where one value alone has too
+// many, a bound on the index. The whole takes NG maxima per thread.
+template <typename T, int NG>
+DEV void top_alternatives(const T *row, long V, const float *gmax, int K,
+                          TopShared &sh, float *top_lp, long *top_ids,
+                          double m, double inv_t, double ln_s, bool none) {
+    const int tid = threadIdx.x, lane = tid % WAVE, wid = tid / WAVE;
+    const int G = (int)((V + GROUP - 1) / GROUP);
+    int turn = 0;
+    if (tid == 0) sh.n_group = sh.n_key = 0;
+    u32 key[NG];
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        const int g = i * BLOCK + tid;
+        key[i] = g < G ? Order<T>::of(gmax[g]) : 0;
+    }
+    u32 bound = 0;  // the K-th largest maximum, all bits below it 0
+    int reach = G;  // how many reach it
+    int KG = K;
+    if (G <= K) {
+        bound = 1;
+        KG = G;
+    } else {
+        for (int bit = Order<T>::BITS - 1; bit >= 0; --bit) {
+            const u32 b = bound | 1u << bit;
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < NG; ++i) n += __popcll(__ballot(key[i] >= b));
+            n = block_count(n, sh, turn);
+            if (n >= K) {
+                bound = b;
+                reach = n;
+                if (n == K) break;
+            }
+        }
+    }
+    // of the groups that equal the bound, those of lowest index
+    int before[NG], quota = BLOCK * NG;
+    if (reach > KG) {
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            above += __popcll(__ballot(key[i] > bound));
+            const int ties = __popcll(__ballot(key[i] == bound));
+            if (lane == 0) sh.ties[i * WAVES + wid] = ties;
+        }
+        quota = KG - block_count(above, sh, turn);
+        int run = 0;
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                if (w == wid) before[i] = run;
+                run += sh.ties[i * WAVES + w];
+            }
+    } else {
+        __syncthreads();  // n_group, n_key
+#pragma unroll
+        for (int i = 0; i < NG; ++i) before[i] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        const u64 ties = __ballot(key[i] == bound);
+        const int nth = before[i] + __popcll(ties & ((1ull << lane) - 1));
+        if (key[i] > bound || (key[i] == bound && nth < quota) ||
+            (reach <= KG && key[i] >= bound))
+            sh.group[atomicAdd(&sh.n_group, 1)] = i * BLOCK + tid;
     }
     __syncthreads();
-    if (threadIdx.x % WAVE == 0) lds[threadIdx.x / WAVE] = v;
+    u32 index_bound = 0xffffffffu;
+    auto collect = [&](u32 order, u32 index, bool valid) {
+        if (valid && (order > bound || (order == bound && index < index_bound))) {
+            const int slot = atomicAdd(&sh.n_key, 1);
+            if (slot < CAP) sh.key[slot] = (u64)order << 32 | ~index;
+        }
+    };
+    for_candidates<T>(row, V, sh, KG, collect);
     __syncthreads();
-    u64 r = lds[0];
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) r = lds[w] > r ? lds[w] : r;
-    return r;
+    int n = sh.n_key;
+    if (n > CAP) {
+        bound = 0;
+        for (int bit = Order<T>::BITS - 1; bit >= 0; --bit) {
+            const u32 b = bound | 1u << bit;
+            int c = 0;
+            for_candidates<T>(row, V, sh, KG, [&](u32 order, u32, bool valid) {
+                c += __popcll(__ballot(valid && order >= b));
+            });
+            c = block_count(c, sh, turn);
+            if (c >= K) {
+                bound = b;
+                n = c;
+                if (c <= CAP) break;
+            }
+        }
+        if (n > CAP) {
+            // more than CAP tokens share the K-th value: `need` of them, the
+            // first ones
+            int above = 0;
+            for_candidates<T>(row, V, sh, KG, [&](u32 order, u32, bool valid) {
+                above += __popcll(__ballot(valid && order > bound));
+            });
+            const int need = K - block_count(above, sh, turn);
+            index_bound = 0;
+            for (int bit = 30; bit >= 0; --bit) {
+                const u32 b = index_bound | 1u << bit;
+                int c = 0;
+                for_candidates<T>(
+                    row, V, sh, KG, [&](u32 order, u32 index, bool valid) {
+                        c += __popcll(__ballot(valid && order == bound &&
+                                               index < b));
+                    });
+                if (block_count(c, sh, turn) <= need) index_bound = b;
+            }
+        }
+        if (tid == 0) sh.n_key = 0;
+        __syncthreads();
+        for_candidates<T>(row, V, sh, KG, collect);
+        __syncthreads();
+        n = sh.n_key;
+    }
+    for (int i = tid; i < n; i += BLOCK) {
+        const u64 mine = sh.key[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += sh.key[j] > mine;
+        if (rank < K) {
+            const u32 index = ~(u32)mine;
+            top_ids[rank] = (long)index;
+            top_lp[rank] = none ? -INFINITY
+                                : (float)(((double)to_f(row[index]) - m) *
+                                              inv_t - ln_s);
+        }
+    }
+    __syncthreads();
 }
 
 // stat[r] = (m, 1/s, H - ln s, 0) against the rounded m*c, what the gradient
 // needs; 1/s is 0 where the row has no finite logit
-template <typename T>
+template <typename T, int NG>
 __global__ __launch_bounds__(BLOCK) void logprobs_join(
     VocabRows g, const float4 *__restrict__ part,
-    const long *__restrict__ tokens, long ignore, int K, float c, double inv_t,
+    const float *__restrict__ gmax, const long *__restrict__ tokens, long ignore, int K, float c, double inv_t,
     float *__restrict__ logprobs, float *__restrict__ entropy,
     float *__restrict__ top_lp, long *__restrict__ top_ids,
     float4 *__restrict__ stat) {
+    constexpr int GPS = WAVE * NVEC * Vec<T>::N / GROUP;  // per stretch
     __shared__ double lds[WAVES];
-    __shared__ u64 lds_k[WAVES];
+    __shared__ TopShared sh;
     const float NEG = -INFINITY;
     for (int r = blockIdx.x; r < g.rows; r += gridDim.x) {
         const long tok = tokens ? tokens[r] : 0;
@@ -335,24 +544,18 @@ __global__ __launch_bounds__(BLOCK) void logprobs_join(
                                (st.t / st.s + st.delta)),
                 0.f);
         }
-        u64 last = ~0ull;
-        for (int k = 0; k < K; ++k) {
-            u64 best = 0;
-            for (long i = threadIdx.x; i < g.V; i += BLOCK) {
-                const u64 key = (u64)order_of(to_f(row[i])) << 32 |
-                                (0xffffffffu - (u32)i);
-                if (key < last && key > best) best = key;
-            }
-            best = block_max_u64(best, lds_k);
-            last = best;
-            if (threadIdx.x == 0) {
-                const u32 i = 0xffffffffu - (u32)best;
-                const float x = to_f(row[i < g.V ? i : 0]);
-                top_lp[(long)r * K + k] =
-                    bad ? NAN
-                        : none ? NEG
-                               : (float)(((double)x - st.m) * inv_t - ln_s);
-                top_ids[(long)r * K + k] = bad ? -1 : (long)i;
+        if (NG > 0) {
+            float *lp_out = top_lp + (long)r * K;
+            long *id_out = top_ids + (long)r * K;
+            if (bad) {
+                for (int k = threadIdx.x; k < K; k += BLOCK) {
+                    lp_out[k] = NAN;
+                    id_out[k] = -1;
+                }
+            } else {
+                top_alternatives<T, (NG > 0 ? NG : 1)>(
+                    row, g.V, gmax + (long)r * g.nseg * GPS, K, sh, lp_out,
+                    id_out, st.m, inv_t, ln_s, none);
             }
         }
         __syncthreads();
@@ -571,17 +774,37 @@ static int row_grid(const VocabRows &g) {
     return g.rows < (1 << 22) ? g.rows : (1 << 22);
 }
 
+template <typename T, int NG>
+static void logprobs_join_t(const VocabRows &g, const VocabLogprobs &a,
+                            float c, hipStream_t stream) {
+    hipLaunchKernelGGL((logprobs_join<T, NG>), dim3(row_grid(g)), dim3(BLOCK),
+                       0, stream, g, (const float4 *)a.part, a.gmax, a.tokens,
+                       a.ignore, a.K, c, 1. / a.temperature, a.logprobs,
+                       a.entropy, a.top_lp, a.top_ids, (float4 *)a.stat);
+}
+
 template <typename T>
 static void logprobs_fwd_t(const VocabRows &g, const VocabLogprobs &a,
                            hipStream_t stream) {
     const float c = (float)(1.4426950408889634 / a.temperature);
-    hipLaunchKernelGGL((vocab_partials<T, true, false>), dim3(wave_grid(g)),
-                       dim3(BLOCK), 0, stream, g, a.tokens, a.ignore, nullptr,
-                       0, c, (float4 *)a.part);
-    hipLaunchKernelGGL((logprobs_join<T>), dim3(row_grid(g)), dim3(BLOCK), 0,
-                       stream, g, (const float4 *)a.part, a.tokens, a.ignore,
-                       a.K, c, 1. / a.temperature, a.logprobs, a.entropy,
-                       a.top_lp, a.top_ids, (float4 *)a.stat);
+    if (a.K == 0) {
+        hipLaunchKernelGGL((vocab_partials<T, true, false, false>),
+                           dim3(wave_grid(g)), dim3(BLOCK), 0, stream, g,
+                           a.tokens, a.ignore, nullptr, 0, c,
+                           (float4 *)a.part, nullptr);
+        logprobs_join_t<T, 0>(g, a, c, stream);
+        return;
+    }
+    hipLaunchKernelGGL((vocab_partials<T, true, false, true>),
+                       dim3(wave_grid(g)), dim3(BLOCK), 0, stream, g,
+                       a.tokens, a.ignore, nullptr, 0, c, (float4 *)a.part,
+                       a.gmax);
+    // maxima per thread; more than VOCAB_MAX_TOP_V tokens are refused before
+    const long per = CDIV(CDIV(g.V, (long)GROUP), (long)BLOCK);
+    if (per <= 4) logprobs_join_t<T, 4>(g, a, c, stream);
+    else if (per <= 8) logprobs_join_t<T, 8>(g, a, c, stream);
+    else if (per <= 16) logprobs_join_t<T, 16>(g, a, c, stream);
+    else logprobs_join_t<T, 32>(g, a, c, stream);
 }
 
 template <typename T>
@@ -589,13 +812,15 @@ static void distill_fwd_t(const VocabRows &g, const VocabDistill &a,
                           hipStream_t stream) {
     const float c = (float)(1.4426950408889634 / a.temperature);
     if (a.bucket)
-        hipLaunchKernelGGL((vocab_partials<T, false, true>),
+        hipLaunchKernelGGL((vocab_partials<T, false, true, false>),
                            dim3(wave_grid(g)), dim3(BLOCK), 0, stream, g,
-                           nullptr, 0, a.ids, a.K, c, (float4 *)a.part);
+                           nullptr, 0, a.ids, a.K, c, (float4 *)a.part,
+                           nullptr);
     else
-        hipLaunchKernelGGL((vocab_partials<T, false, false>),
+        hipLaunchKernelGGL((vocab_partials<T, false, false, false>),
                            dim3(wave_grid(g)), dim3(BLOCK), 0, stream, g,
-                           nullptr, 0, nullptr, 0, c, (float4 *)a.part);
+                           nullptr, 0, nullptr, 0, c, (float4 *)a.part,
+                           nullptr);
     hipLaunchKernelGGL((distill_join<T>), dim3(row_grid(g)), dim3(BLOCK), 0,
                        stream, g, (const float4 *)a.part, a.teacher_lp, a.ids,
                        a.K, a.bucket, c, 1. / a.temperature, a.loss, a.q,
@@ -616,6 +841,8 @@ static void grad_t(const VocabRows &g, const VocabGrad &a, int distill,
 extern "C" int vocab_segment(int dtype) {
     return WAVE * NVEC * (dtype == VOCAB_FP32 ? 4 : 8);
 }
+extern "C" int vocab_group(void) { return GROUP; }
+static_assert(32 * BLOCK * GROUP == VOCAB_MAX_TOP_V, "limits agree");
 
 extern "C" void logprobs_fwd_launch(const VocabRows *g, const VocabLogprobs *a,
                                     int dtype, hipStream_t stream) {

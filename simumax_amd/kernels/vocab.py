@@ -33,6 +33,7 @@ from torch.autograd.function import once_differentiable
 from . import insitu
 
 MAX_TOPK = 256       # VOCAB_MAX_K in csrc/vocab.h
+MAX_TOP_V = 524288   # VOCAB_MAX_TOP_V there
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -192,7 +193,8 @@ def token_logprobs(logits, tokens=None, topk=0, temperature=1.0,
     logits [..., V]; tokens [...] int64, or None where only the entropies and
     alternatives are wanted. A row whose token is ``ignore_index`` is left
     out whole: zeros, ids of -1, no gradient, and it is not read. Of equal
-    logits the one of lowest index comes first. ``topk`` <= 256.
+    logits the one of lowest index comes first. ``topk`` <= 256, and where it
+    is not 0, V <= 524288.
 
     Returns ``TokenLogprobs(logprobs, entropy, top_logprobs, top_ids)``, of
     which the first three are differentiable; what was not asked for is
@@ -202,6 +204,9 @@ def token_logprobs(logits, tokens=None, topk=0, temperature=1.0,
     if not 0 <= topk <= min(MAX_TOPK, V):
         raise ValueError(f"topk must be in [0, {min(MAX_TOPK, V)}] for a "
                          f"vocabulary of {V}, not {topk}")
+    if topk and V > MAX_TOP_V:
+        raise ValueError(f"top alternatives of a vocabulary of {V}: at most "
+                         f"{MAX_TOP_V}")
     if tokens is not None:
         _check_ids("tokens", tokens, logits.shape[:-1], logits.device)
         tokens = tokens.contiguous()

@@ -243,6 +243,7 @@ def test_top_alternatives_feed_distillation():
     (dict(logits=torch.zeros(2, 0)), ValueError),
     (dict(logits=torch.zeros(())), ValueError),
     (dict(logits=torch.zeros(2, 1000), topk=257), ValueError),
+    (dict(logits=torch.zeros(2, 524289), topk=1), ValueError),
 ])
 def test_logprobs_refuses(kw, err):
     args = dict(logits=torch.zeros(2, 17),
