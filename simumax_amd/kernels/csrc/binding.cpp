@@ -332,6 +332,7 @@ static bool vocab_rows(const torch::Tensor &x, VocabRows *g) {
     g->inner = (int)std::max<int64_t>(dims[1].first, 1);
     const int seg = vocab_segment(vocab_dtype(x));
     g->nseg = (int)((V + seg - 1) / seg);
+    TORCH_CHECK(rows * g->nseg < (1ll << 31), rows, " rows of ", V, " logits");
     return true;
 }
 
