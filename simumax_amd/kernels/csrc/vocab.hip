@@ -44,6 +44,7 @@ typedef unsigned long long u64;
 // against 5.2).
 typedef u32 u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_mem __attribute__((aligned(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
@@ -106,11 +107,14 @@ template <> DEV void Vec<float>::put(int i, float a, float b) {
     w[i + 1] = __float_as_uint(b);
 }
 template <> DEV void Vec<bf16>::put(int i, float a, float b) {
-    w[i >> 1] = (u32)f2bf(a) | ((u32)f2bf(b) << 16);
+    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+    const f32x2 f = {a, b};
+    w[i >> 1] = __builtin_bit_cast(u32, __builtin_convertvector(f, bf2));
 }
 template <> DEV void Vec<__half>::put(int i, float a, float b) {
-    w[i >> 1] = (u32)__half_as_ushort(__float2half(a)) |
-                ((u32)__half_as_ushort(__float2half(b)) << 16);
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const f32x2 f = {a, b};
+    w[i >> 1] = __builtin_bit_cast(u32, __builtin_convertvector(f, h2));
 }
 
 // the two running patterns of Vec::widen, and what they say
@@ -135,13 +139,36 @@ template <> DEV float from_pattern<__half>(u32 b) {
     return __half2float(__ushort_as_half((unsigned short)b));
 }
 
-// `at` counts elements from the row's start; lanes past its end see -inf
-template <typename T>
-DEV Vec<T> load_vec(const T *row, long at, long V) {
+template <typename T> DEV u32 pad_word() {  // -inf, once or twice
+    return sizeof(T) == 4                       ? 0xff800000u
+           : std::is_same<T, bf16>::value ? 0xff80ff80u : 0xfc00fc00u;
+}
+
+// A vector of which `past` elements lie behind the row's end, taken from the
+// row's last 16 bytes: moved down, and -inf behind.
+template <typename T> DEV void shift_in_pad(Vec<T> &v, int past) {
+    const u32 pad = pad_word<T>();
+    if constexpr (sizeof(T) == 2) {
+        if (past & 1) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                v.w[k] = __builtin_amdgcn_alignbit(k < 3 ? v.w[k + 1] : pad,
+                                                   v.w[k], 16);
+        }
+    }
+    const int words = past * (int)sizeof(T) / 4;
+    if (words & 1) v.w = (u32x4){v.w[1], v.w[2], v.w[3], pad};
+    if (words & 2) v.w = (u32x4){v.w[2], v.w[3], pad, pad};
+    if (words & 4) v.w = (u32x4){pad, pad, pad, pad};
+}
+
+// `at` counts elements from the row's start; elements past its end are -inf
+template <typename T> DEV Vec<T> load_vec(const T *row, long at, long V) {
     constexpr int N = Vec<T>::N;
     Vec<T> v;
-    if (at + N <= V) {
-        v.load(row + at);
+    if (V >= N) {
+        v.load(row + min(at, V - N));
+        shift_in_pad(v, (int)min(max(at + N - V, 0l), (long)N));
     } else {
         float f[N];
 #pragma unroll
@@ -153,36 +180,53 @@ DEV Vec<T> load_vec(const T *row, long at, long V) {
     return v;
 }
 
-// a wave's stretch of a row. Only a row's last one can be cut short: the
-// others' loads are all in flight at once, without a test.
+// a wave's stretch of a row; only a row's last one can be cut short
 template <typename T>
 DEV void load_stretch(const T *row, long lo, long V, int lane,
                       Vec<T> (&v)[NVEC]) {
     constexpr int N = Vec<T>::N;
-    if (lo + WAVE * NVEC * N <= V) {
+    constexpr int SEG = WAVE * NVEC * N;
+    if (lo + SEG <= V) {
         const T *p = row + lo + lane * N;
 #pragma unroll
-        for (int j = 0; j < NVEC; ++j)
-            v[j].stream_in(p + j * WAVE * N);
-    } else {
+        for (int j = 0; j < NVEC; ++j) v[j].stream_in(p + j * WAVE * N);
+    } else if (V >= N) {
+        const int rest = (int)(V - lo);  // below SEG
 #pragma unroll
-        for (int j = 0; j < NVEC; ++j)
-            v[j] = load_vec(row, lo + (long)(j * WAVE + lane) * N, V);
+        for (int j = 0; j < NVEC; ++j) {
+            const int at = (j * WAVE + lane) * N;
+            v[j].load(row + lo + min(at, rest - N));
+        }
+#pragma unroll
+        for (int j = 0; j < NVEC; ++j) {
+            const int at = (j * WAVE + lane) * N;
+            shift_in_pad(v[j], min(max(at + N - rest, 0), N));
+        }
+    } else {
+        v[0] = load_vec(row, (long)lane * N, V);
+#pragma unroll
+        for (int j = 1; j < NVEC; ++j) v[j].w = pad_word<T>();
     }
 }
 
 template <typename T>
-DEV void store_vec(T *row, long at, long V, const float *f) {
+DEV void store_vec(T *row, long at, long V, const float *f, bool whole) {
     constexpr int N = Vec<T>::N;
-    if (at + N <= V) {
-        Vec<T> v;
+    Vec<T> v;
 #pragma unroll
-        for (int i = 0; i < N; i += 2) v.put(i, f[i], f[i + 1]);
+    for (int i = 0; i < N; i += 2) v.put(i, f[i], f[i + 1]);
+    if (whole || at + N <= V) {  // whole: the same for all lanes
         v.stream_out(row + at);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (at + i < V) row[at + i] = from_f<T>(f[i]);
+            if (at + i < V) {
+                if constexpr (sizeof(T) == 4)
+                    row[at + i] = __uint_as_float(v.w[i]);
+                else
+                    ((unsigned short *)row)[at + i] =
+                        (unsigned short)(v.w[i >> 1] >> (i & 1) * 16);
+            }
     }
 }
 
@@ -207,12 +251,6 @@ DEV float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
 // part of the exponent (logits at a type's lowest or highest value) the
 // difference is taken first.
 DEV bool by_product(float mc) { return fabsf(mc) < 0x1p20f; }
-
-// Not below -300: 2^-300 is 0 and (-inf) * 0 would be NaN.
-DEV float diff2_safe(float x, float m, float mc, float c) {
-    float d = by_product(mc) ? fmaf(x, c, -mc) : (x - m) * c;
-    return d < -300.f ? -300.f : d;
-}
 
 // sums and maxima over a wave, in every lane: within 16 lanes by data
 // movement in the operand, then the four rows through scalar registers
@@ -802,24 +840,34 @@ __global__ __launch_bounds__(BLOCK) void distill_join(
 
 // ---- gradients -------------------------------------------------------------
 // d x_j = p_j (a + b ln(p_j s)) + what is given for single tokens, one wave per
-// stretch. Single tokens: a list of at most K entries of the row that fall
-// into this stretch, compacted into LDS in the row's order, with one bit per
-// element so that the rest of the stretch never looks at it. The same token
-// given twice is added twice, in order.
+// stretch, in one pass over packed registers: a product, an exponential and
+// one or three more operations per element beside 4 or 8 bytes.
+//
+// Single tokens (the given one, alternatives with a gradient, a teacher's
+// entries) are not looked for in the pass: the entries that fall into the
+// stretch are gathered into LDS in the row's order, and after the stretch is
+// written, and its stores have arrived, each one's lane computes its token
+// anew and writes it once more. The same token given twice is added up by its
+// first entry's lane, in order.
 template <typename T, bool DISTILL>
 __global__ __launch_bounds__(BLOCK) void vocab_grad(
     VocabRows g, VocabGrad a, T *__restrict__ out) {
     constexpr int N = Vec<T>::N;
     constexpr int SEG = WAVE * NVEC * N;
-    __shared__ u32 bits[WAVES][SEG / 32];
-    __shared__ int list_at[WAVES][VOCAB_MAX_K + 1];
-    __shared__ float list_val[WAVES][VOCAB_MAX_K + 1];
-    const int lane = threadIdx.x % WAVE, wid = threadIdx.x / WAVE;
-    const long total = (long)g.rows * g.nseg;
-    for (long w = (long)blockIdx.x * WAVES + wid; w < total;
-         w += (long)gridDim.x * WAVES) {
-        const int r = (int)(w / g.nseg), seg = (int)(w - (long)r * g.nseg);
+    __shared__ u32 bits_all[WAVES][SEG / 32];
+    __shared__ int at_all[WAVES][VOCAB_MAX_K + 1];
+    __shared__ float val_all[WAVES][VOCAB_MAX_K + 1];
+    const int lane = threadIdx.x % WAVE;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    u32 *bits = bits_all[wid];
+    int *list_at = at_all[wid];
+    float *list_val = val_all[wid];
+    const float *vals = DISTILL ? a.q : a.d_top;
+    const u32 total = (u32)g.rows * g.nseg;  // below 2^31, as is w's step
+    for (u32 w = wave_index(); w < total; w += gridDim.x * WAVES) {
+        const int r = w / (u32)g.nseg, seg = w - (u32)r * g.nseg;
         const long lo = (long)seg * SEG;
+        const bool whole = lo + SEG <= g.V;
         T *orow = out + (long)r * g.V;
         const float4 st = a.stat[r];
         bool skip = st.y == 0.f;
@@ -827,48 +875,47 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
         const long tok = !DISTILL && a.tokens ? a.tokens[r] : -1;
         if (!DISTILL && a.tokens && tok == a.ignore) skip = true;
         if (skip) {
-            float zero[N] = {};
-#pragma unroll
-            for (int j = 0; j < NVEC; ++j) {
-                const long at = lo + (long)(j * WAVE + lane) * N;
-                store_vec(orow, at, g.V, zero);
-            }
+            const float zero[N] = {};
+#pragma unroll 1
+            for (int j = 0; j < NVEC; ++j)
+                store_vec(orow, lo + (long)(j * WAVE + lane) * N, g.V, zero,
+                          whole);
             continue;
         }
-        for (int i = lane; i < SEG / 32; i += WAVE) bits[wid][i] = 0;
-        wave_sync();
-        // coefficients of p_j: a_in for listed tokens, a_out for the others
-        float a_in, a_out, b = 0.f, scale = a.inv_t;
+        const T *row = row_ptr<T>(g, r);
+        Vec<T> v[NVEC];
+        load_stretch(row, lo, g.V, lane, v);
+        // e = 2^((x - m) c) counts k_out (k_in where listed) + k_d * exponent
         int n = 0;
+        float k_in, k_out, k_d = 0.f, scale = a.inv_t;
         if (DISTILL) {
             scale *= a.d_row[r];
-            a_in = st.z;
-            a_out = st.w;
+            k_in = st.z;
+            k_out = st.w;
         } else {
             float gs = 0.f;
             if (a.d_row && a.tokens) {
                 const float gr = a.d_row[r];
                 gs = tok >= 0 && tok < g.V ? gr : NAN;
                 const long at = tok - lo;
-                if (at >= 0 && at < SEG) {
+                if (at >= 0 && at < SEG && tok < g.V) {
                     if (lane == 0) {
-                        bits[wid][at >> 5] |= 1u << (at & 31);
-                        list_at[wid][0] = (int)at;
-                        list_val[wid][0] = gr;
+                        list_at[0] = (int)at;
+                        list_val[0] = gr;
                     }
                     n = 1;
                 }
             }
-            float gk = 0.f;
-            if (a.d_top)
+            if (a.d_top) {
+                float gk = 0.f;
                 for (int k = lane; k < a.K; k += WAVE)
                     gk += a.d_top[(long)r * a.K + k];
-            gs += wave_sum(gk);
-            if (a.d_entropy) b = -a.d_entropy[r];
-            a_in = a_out = b * st.z - gs;
+                gs += sum_wave(gk);
+            }
+            if (a.d_entropy) k_d = -a.d_entropy[r];
+            k_in = k_out = k_d * st.z - gs;
+            k_d *= 0.69314718f;
         }
-        wave_sync();
-        const float *vals = DISTILL ? a.q : a.d_top;
         if (vals) {
             for (int k0 = 0; k0 < a.K; k0 += WAVE) {
                 const int k = k0 + lane;
@@ -876,49 +923,86 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
                 const bool mine = at >= 0 && at < SEG && at + lo < g.V;
                 const u64 who = __ballot(mine);
                 if (mine) {
-                    const int slot =
-                        n + __popcll(who & ((1ull << lane) - 1));
+                    const int slot = n + __popcll(who & ((1ull << lane) - 1));
                     const float val = vals[(long)r * a.K + k];
-                    list_at[wid][slot] = (int)at;
-                    list_val[wid][slot] = DISTILL ? -val : val;
-                    atomicOr(&bits[wid][at >> 5], 1u << (at & 31));
+                    list_at[slot] = (int)at;
+                    list_val[slot] = DISTILL ? -val : val;
                 }
                 n += __popcll(who);
             }
         }
         wave_sync();
-        const T *row = row_ptr<T>(g, r);
-        Vec<T> v[NVEC];
+        const float mc = st.x * a.c, u = st.y * scale;
+        const float u_out = k_out * u, u_d = k_d * u;
+        const bool product = by_product(mc);
+        auto grad = [&](float d, float uk) {
+            // 2^-300 is 0, and (-inf) * 0 would be NaN
+            if (!DISTILL) uk = fmaf(u_d, fmaxf(d, -300.f), uk);
+            return exp2_hw(d) * uk;
+        };
+        if (product) {
 #pragma unroll
-        for (int j = 0; j < NVEC; ++j)
-            v[j] = load_vec(row, lo + (long)(j * WAVE + lane) * N, g.V);
-        const float mc = st.x * a.c;
-#pragma unroll
-        for (int j = 0; j < NVEC; ++j) {
-            const int at = (j * WAVE + lane) * N;
-            const u32 in =
-                (bits[wid][at >> 5] >> (at & 31)) & ((1u << N) - 1);
-            float f[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float d = diff2_safe(v[j].get(i), st.x, mc, a.c);
-                const float p = exp2_hw(d) * st.y;
-                float k = a_out;
-                if (!DISTILL) k = fmaf(b * 0.69314718f, d, k);
-                else if (in >> i & 1) k = a_in;
-                f[i] = p * k;
-            }
-            if (in) {
+            for (int j = 0; j < NVEC; ++j) {
+                float f[N];
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (in >> i & 1)
-                        for (int e = 0; e < n; ++e)
-                            if (list_at[wid][e] == at + i)
-                                f[i] += list_val[wid][e];
+                    f[i] = grad(fmaf(v[j].get(i), a.c, -mc), u_out);
+                store_vec(orow, lo + (long)(j * WAVE + lane) * N, g.V, f,
+                          whole);
             }
+        } else {
+#pragma unroll 1
+            for (int j = 0; j < NVEC; ++j) {
+                const long at = lo + (long)(j * WAVE + lane) * N;
+                const Vec<T> x = load_vec(row, at, g.V);
+                float f[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) f[i] *= scale;
-            store_vec(orow, lo + at, g.V, f);
+                for (int i = 0; i < N; ++i)
+                    f[i] = grad((x.get(i) - st.x) * a.c, u_out);
+                store_vec(orow, at, g.V, f, whole);
+            }
+        }
+        if (n > 0) {
+            // is a token listed twice?
+            u64 twice = 0;
+            if (n > 1) {
+                for (int i = lane; i < SEG / 32; i += WAVE) bits[i] = 0;
+                wave_sync();
+                for (int k0 = 0; k0 < n; k0 += WAVE) {
+                    bool seen = false;
+                    if (k0 + lane < n) {
+                        const int at = list_at[k0 + lane];
+                        const u32 bit = 1u << (at & 31);
+                        seen = atomicOr(&bits[at >> 5], bit) & bit;
+                    }
+                    twice |= __ballot(seen);
+                }
+            }
+            for (int k0 = 0; k0 < n; k0 += WAVE) {
+                const int k = k0 + lane;
+                const int at = k < n ? list_at[k] : -1;
+                float val = k < n ? list_val[k] : 0.f;
+                bool first = k < n;
+                if (twice) {
+                    val = 0.f;
+                    for (int e = 0; e < n; ++e) {
+                        const bool same = list_at[e] == at;
+                        if (same) val += list_val[e];
+                        if (same && e < k) first = false;
+                    }
+                }
+                float f = 0.f;
+                if (first) {
+                    const float x = to_f(row[lo + at]);
+                    f = fmaf(val, scale,
+                             grad(product ? fmaf(x, a.c, -mc)
+                                          : (x - st.x) * a.c,
+                                  k_in * u));
+                }
+                // the stretch's own stores are to arrive first
+                if (k0 == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                if (first) orow[lo + at] = from_f<T>(f);
+            }
         }
         wave_sync();
     }
