@@ -15,7 +15,8 @@
 // Three launches, none of which synchronises with the host:
 //   partials: one wave per 16-byte x 64 lanes x 8 stretch of a row, held in
 //             registers: one read for the maximum and the sums;
-//   join:     one workgroup per row: statistics, top alternatives, loss;
+//   join:     one wave per row (one workgroup where top alternatives are
+//             asked): statistics, loss;
 //   grad:     one wave per stretch again: p from the statistics, plus what
 //             the given tokens or the teacher's entries add.
 // No floating-point atomics: the same input gives the same bits.
@@ -304,16 +305,31 @@ DEV u32 min_wave(u32 v) {
                min((u32)lane_i(v, 32), (u32)lane_i(v, 48)));
 }
 
-DEV double block_sum_d(double v, double *lds) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, WAVE);
-    __syncthreads();
-    if (threadIdx.x % WAVE == 0) lds[threadIdx.x / WAVE] = v;
-    __syncthreads();
-    double r = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) r += lds[w];
-    return r;
+DEV double lane_d(double v, int lane) {
+    const u64 b = __builtin_bit_cast(u64, v);
+    const u64 lo = (u32)lane_i((int)(u32)b, lane);
+    const u64 hi = (u32)lane_i((int)(u32)(b >> 32), lane);
+    return __builtin_bit_cast(double, hi << 32 | lo);
+}
+template <int CTRL> DEV double dpp_d(double v) {
+    const u64 b = __builtin_bit_cast(u64, v);
+    const u64 lo = dpp_i<CTRL>((u32)b), hi = dpp_i<CTRL>((u32)(b >> 32));
+    return __builtin_bit_cast(double, hi << 32 | lo);
+}
+DEV double sum_wave_d(double v) {
+    v += dpp_d<DPP_XOR1>(v);
+    v += dpp_d<DPP_XOR2>(v);
+    v += dpp_d<DPP_HALF_MIRROR>(v);
+    v += dpp_d<DPP_MIRROR>(v);
+    return (lane_d(v, 0) + lane_d(v, 16)) + (lane_d(v, 32) + lane_d(v, 48));
+}
+DEV float max_wave_f(float v) {
+    v = fmaxf(v, dpp<DPP_XOR1>(v));
+    v = fmaxf(v, dpp<DPP_XOR2>(v));
+    v = fmaxf(v, dpp<DPP_HALF_MIRROR>(v));
+    v = fmaxf(v, dpp<DPP_MIRROR>(v));
+    return fmaxf(fmaxf(lane_f(v, 0), lane_f(v, 16)),
+                 fmaxf(lane_f(v, 32), lane_f(v, 48)));
 }
 
 // ---- partials --------------------------------------------------------------
@@ -467,19 +483,18 @@ struct RowStat {
                        // 2^delta times too large
 };
 
-// every thread gets the row's statistics; sums in a fixed order, in 64 bits
-DEV RowStat join_parts(const float4 *p, int nseg, float c, double *lds) {
-    __shared__ float redm[WAVES];
+// one wave joins a row's stretches, each lane's in order, in 64 bits
+DEV RowStat join_parts(const float4 *p, int nseg, float c, int lane) {
     float m = -INFINITY;
-    for (int i = threadIdx.x; i < nseg; i += BLOCK) m = fmaxf(m, p[i].x);
-    m = block_max<BLOCK>(m, redm);
+    for (int i = lane; i < nseg; i += WAVE) m = fmaxf(m, p[i].x);
+    m = max_wave_f(m);
     RowStat st;
     st.m = m == -INFINITY ? 0.f : m;
     const float mc = st.m * c;
     const double exact = (double)st.m * c;
     st.delta = by_product(mc) ? exact - mc : 0.;
     double s = 0, t = 0, s_in = 0;
-    for (int i = threadIdx.x; i < nseg; i += BLOCK) {
+    for (int i = lane; i < nseg; i += WAVE) {
         const float4 q = p[i];
         const float qm = q.x == -INFINITY ? 0.f : q.x;
         // against each stretch's own rounded reference, where there is one
@@ -492,9 +507,9 @@ DEV RowStat join_parts(const float4 *p, int nseg, float c, double *lds) {
         s_in += q.w * f;
         t += (q.z + d * ((double)q.y + q.w)) * f;
     }
-    st.s = block_sum_d(s, lds);
-    st.s_in = block_sum_d(s_in, lds);
-    st.t = block_sum_d(t, lds);
+    st.s = sum_wave_d(s);
+    st.s_in = sum_wave_d(s_in);
+    st.t = sum_wave_d(t);
     return st;
 }
 
@@ -691,75 +706,114 @@ DEV void top_alternatives(const T *row, long V, const float *gmax, int K,
     __syncthreads();
 }
 
-// stat[r] = (m, 1/s, H - ln s, 0) against the rounded m*c, what the gradient
-// needs; 1/s is 0 where the row has no finite logit
-template <typename T, int NG>
+struct RowOut {
+    double m, ln_s;
+    bool none, bad;  // no finite logit; NaN or +inf among them
+};
+
+// One wave: a row's log probability, entropy and stat[r] =
+// (m, 1/s, H - ln s, 0) against the rounded m*c, what the gradient needs;
+// 1/s is 0 where the row has no finite logit.
+template <typename T>
+DEV RowOut logprobs_row(const VocabRows &g, const float4 *part, int r,
+                        const long *tokens, float c, double inv_t,
+                        float *logprobs, float *entropy, float4 *stat,
+                        int lane, bool write) {
+    const RowStat st = join_parts(part + (long)r * g.nseg, g.nseg, c, lane);
+    RowOut o;
+    o.m = st.m;
+    o.none = st.s == 0;
+    o.bad = !(st.s < INFINITY);
+    o.ln_s = log(st.s);
+    if (write && lane == 0) {
+        if (tokens) {
+            const long tok = tokens[r];
+            float lp = NAN;
+            if (tok >= 0 && tok < g.V && !o.bad)
+                lp = o.none ? -INFINITY
+                            : (float)(((double)to_f(row_ptr<T>(g, r)[tok]) -
+                                       o.m) * inv_t - o.ln_s);
+            logprobs[r] = lp;
+        }
+        const double ln2 = 0.6931471805599453, mean = st.t / st.s;
+        entropy[r] = o.none ? 0.f
+                     : o.bad ? NAN : (float)(o.ln_s - ln2 * mean);
+        stat[r] = make_float4(
+            st.m, o.none ? 0.f : (float)(exp2(-st.delta) / st.s),
+            o.none ? 0.f : (float)(-ln2 * (mean + st.delta)), 0.f);
+    }
+    return o;
+}
+
+// without alternatives: one wave per row
+template <typename T>
 __global__ __launch_bounds__(BLOCK) void logprobs_join(
     VocabRows g, const float4 *__restrict__ part,
-    const float *__restrict__ gmax, const long *__restrict__ tokens, long ignore, int K, float c, double inv_t,
+    const long *__restrict__ tokens, long ignore, float c, double inv_t,
     float *__restrict__ logprobs, float *__restrict__ entropy,
-    float *__restrict__ top_lp, long *__restrict__ top_ids,
     float4 *__restrict__ stat) {
+    const int lane = threadIdx.x % WAVE;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    for (u32 r = blockIdx.x * WAVES + wid; r < (u32)g.rows;
+         r += gridDim.x * WAVES) {
+        if (tokens && tokens[r] == ignore) {
+            if (lane == 0) {
+                logprobs[r] = 0.f;
+                entropy[r] = 0.f;
+                stat[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            continue;
+        }
+        logprobs_row<T>(g, part, (int)r, tokens, c, inv_t, logprobs, entropy,
+                        stat, lane, true);
+    }
+}
+
+// with alternatives: one workgroup per row
+template <typename T, int NG>
+__global__ __launch_bounds__(BLOCK) void logprobs_top_join(
+    VocabRows g, const float4 *__restrict__ part,
+    const float *__restrict__ gmax, const long *__restrict__ tokens,
+    long ignore, int K, float c, double inv_t, float *__restrict__ logprobs,
+    float *__restrict__ entropy, float *__restrict__ top_lp,
+    long *__restrict__ top_ids, float4 *__restrict__ stat) {
     constexpr int GPS = WAVE * NVEC * Vec<T>::N / GROUP;  // per stretch
-    __shared__ double lds[WAVES];
     __shared__ TopShared sh;
-    const float NEG = -INFINITY;
+    const int lane = threadIdx.x % WAVE;
     for (int r = blockIdx.x; r < g.rows; r += gridDim.x) {
-        const long tok = tokens ? tokens[r] : 0;
-        if (tokens && tok == ignore) {
+        float *lp_out = top_lp + (long)r * K;
+        long *id_out = top_ids + (long)r * K;
+        if (tokens && tokens[r] == ignore) {
             if (threadIdx.x == 0) {
                 logprobs[r] = 0.f;
                 entropy[r] = 0.f;
                 stat[r] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
             for (int k = threadIdx.x; k < K; k += BLOCK) {
-                top_lp[(long)r * K + k] = 0.f;
-                top_ids[(long)r * K + k] = -1;
+                lp_out[k] = 0.f;
+                id_out[k] = -1;
             }
             continue;
         }
-        const T *row = row_ptr<T>(g, r);
-        const RowStat st = join_parts(part + (long)r * g.nseg, g.nseg, c, lds);
-        const bool none = st.s == 0, bad = !(st.s < INFINITY);
-        const double ln_s = log(st.s);
-        const float H = none ? 0.f
-                        : bad ? NAN
-                              : (float)(ln_s - 0.6931471805599453 * st.t / st.s);
-        if (threadIdx.x == 0) {
-            if (tokens) {
-                float lp = NAN;
-                if (tok >= 0 && tok < g.V && !bad)
-                    lp = none ? NEG
-                              : (float)(((double)to_f(row[tok]) - st.m) * inv_t -
-                                        ln_s);
-                logprobs[r] = lp;
+        // every wave joins for itself
+        const RowOut o = logprobs_row<T>(g, part, r, tokens, c, inv_t,
+                                         logprobs, entropy, stat, lane,
+                                         threadIdx.x < WAVE);
+        if (o.bad) {
+            for (int k = threadIdx.x; k < K; k += BLOCK) {
+                lp_out[k] = NAN;
+                id_out[k] = -1;
             }
-            entropy[r] = H;
-            stat[r] = make_float4(
-                st.m, none ? 0.f : (float)(exp2(-st.delta) / st.s),
-                none ? 0.f
-                     : (float)(-0.6931471805599453 *
-                               (st.t / st.s + st.delta)),
-                0.f);
+        } else {
+            top_alternatives<T, NG>(row_ptr<T>(g, r), g.V,
+                                    gmax + (long)r * g.nseg * GPS, K, sh,
+                                    lp_out, id_out, o.m, inv_t, o.ln_s,
+                                    o.none);
         }
-        if (NG > 0) {
-            float *lp_out = top_lp + (long)r * K;
-            long *id_out = top_ids + (long)r * K;
-            if (bad) {
-                for (int k = threadIdx.x; k < K; k += BLOCK) {
-                    lp_out[k] = NAN;
-                    id_out[k] = -1;
-                }
-            } else {
-                top_alternatives<T, (NG > 0 ? NG : 1)>(
-                    row, g.V, gmax + (long)r * g.nseg * GPS, K, sh, lp_out,
-                    id_out, st.m, inv_t, ln_s, none);
-            }
-        }
-        __syncthreads();
     }
 }
 
+// One wave per row, up to VOCAB_MAX_K / 64 entries per lane.
 // stat[r] = (m, 1/s, a_in, a_out): the gradient of a student's logit is
 // p_j a_in - sum of its q  inside the teacher's entries, p_j a_out outside.
 // Both 0 mark a row without entries. q [rows, K] is kept for the gradient.
@@ -769,50 +823,76 @@ __global__ __launch_bounds__(BLOCK) void distill_join(
     const float *__restrict__ tlp, const long *__restrict__ ids, int K,
     int bucket, float c, double inv_t, float *__restrict__ loss,
     float *__restrict__ q_out, float4 *__restrict__ stat) {
-    __shared__ double lds[WAVES];
-    for (int r = blockIdx.x; r < g.rows; r += gridDim.x) {
-        const T *row = row_ptr<T>(g, r);
-        // K <= BLOCK: one entry per thread
-        const bool held = (int)threadIdx.x < K &&
-                          ids[(long)r * K + threadIdx.x] >= 0;
-        const long id = held ? ids[(long)r * K + threadIdx.x] : 0;
-        const double l = held ? (double)tlp[(long)r * K + threadIdx.x] : 0.;
-        double q = held ? exp(l) : 0.;
-        const bool wrong = held && id >= g.V;
-        const int any = __syncthreads_or(held ? 1 : 0);
-        const int err = __syncthreads_or(wrong ? 1 : 0);
-        double total = block_sum_d(q, lds);
-        double q_rest = 0., log_norm = 0., mass;
+    constexpr int EPL = VOCAB_MAX_K / WAVE;
+    const int lane = threadIdx.x % WAVE;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    for (u32 r = blockIdx.x * WAVES + wid; r < (u32)g.rows;
+         r += gridDim.x * WAVES) {
+        const T *row = row_ptr<T>(g, (int)r);
+        long id[EPL];
+        float l[EPL], x[EPL];
+        double q[EPL], total = 0.;
+        bool any = false, wrong = false;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            const int k = e * WAVE + lane;
+            id[e] = -1;
+            l[e] = x[e] = 0.f;
+            if (k < K) {
+                id[e] = ids[(long)r * K + k];
+                l[e] = tlp[(long)r * K + k];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            const bool held = id[e] >= 0, in = id[e] < g.V;
+            if (held && in) x[e] = to_f(row[id[e]]);
+            any |= held;
+            wrong |= held && !in;
+            q[e] = 0.;
+            if (__ballot(held)) q[e] = held ? exp((double)l[e]) : 0.;
+            total += q[e];
+        }
+        any = __ballot(any) != 0;
+        wrong = __ballot(wrong) != 0;
+        total = sum_wave_d(total);
+        double q_rest = 0., log_norm = 0., scale = 1., mass;
         if (bucket) {
             q_rest = total < 1. ? 1. - total : 0.;
             mass = total + q_rest;
         } else {
             // not `total > 0`: NaN has to stay NaN
             log_norm = total == 0. ? 0. : log(total);
-            q = total == 0. ? 0. : q / total;
+            scale = total == 0. ? 0. : 1. / total;
             mass = total == 0. ? 0. : total / total;
         }
-        if ((int)threadIdx.x < K) q_out[(long)r * K + threadIdx.x] = (float)q;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            q[e] *= scale;
+            const int k = e * WAVE + lane;
+            if (k < K) q_out[(long)r * K + k] = (float)q[e];
+        }
         if (!any || (!bucket && total == 0.)) {
-            if (threadIdx.x == 0) {
+            if (lane == 0) {
                 loss[r] = 0.f;
                 stat[r] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
             continue;
         }
-        const RowStat st = join_parts(part + (long)r * g.nseg, g.nseg, c, lds);
+        const RowStat st = join_parts(part + (long)r * g.nseg, g.nseg, c, lane);
         const double s = st.s + st.s_in;
         const bool none = s == 0, bad = !(s < INFINITY);
         const double ln_s = log(s);
-        double term = 0.;
-        if (held && !wrong && q != 0.) {
-            const double x = (double)to_f(row[id]);
-            const double lp = none || x == -INFINITY
-                                  ? -INFINITY
-                                  : (x - st.m) * inv_t - ln_s;
-            term = q * ((l - log_norm) - lp);
-        }
-        double sum = block_sum_d(term, lds);
+        double sum = 0.;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e)
+            if (id[e] >= 0 && id[e] < g.V && q[e] != 0.) {
+                const double lp = none || x[e] == -INFINITY
+                                      ? -INFINITY
+                                      : ((double)x[e] - st.m) * inv_t - ln_s;
+                sum += q[e] * (((double)l[e] - log_norm) - lp);
+            }
+        sum = sum_wave_d(sum);
         double ratio = 0.;
         if (bucket && q_rest > 0.) {
             // entries that cover every token with mass leave no room for
@@ -820,21 +900,20 @@ __global__ __launch_bounds__(BLOCK) void distill_join(
             // rounding then counts as none
             const double p_rest = none ? 0. : st.s / s;
             if (p_rest > 0.) {
-                sum += q_rest * (log(q_rest) - log(p_rest));
                 ratio = q_rest / p_rest;
+                sum += q_rest * log(ratio);
             } else if (q_rest > 0x1p-20) {
                 sum = INFINITY;
             }
         }
-        if (threadIdx.x == 0) {
-            const bool nan = bad || err;
+        if (lane == 0) {
+            const bool nan = bad || wrong;
             loss[r] = nan ? NAN : (float)sum;
             stat[r] = make_float4(st.m,
                                   none ? 0.f : (float)(exp2(-st.delta) / s),
                                   nan ? NAN : (float)mass,
                                   nan ? NAN : (float)(mass - ratio));
         }
-        __syncthreads();
     }
 }
 
@@ -1014,17 +1093,18 @@ static int wave_grid(const VocabRows &g) {
     const long blocks = CDIV((long)g.rows * g.nseg, (long)WAVES);
     return (int)(blocks < (1l << 22) ? CDIV(blocks, 8) * 8 : (1l << 22));
 }
-static int row_grid(const VocabRows &g) {
-    return g.rows < (1 << 22) ? g.rows : (1 << 22);
+static int row_grid(long blocks) {
+    return (int)(blocks < (1l << 22) ? blocks : (1l << 22));
 }
 
 template <typename T, int NG>
-static void logprobs_join_t(const VocabRows &g, const VocabLogprobs &a,
-                            float c, hipStream_t stream) {
-    hipLaunchKernelGGL((logprobs_join<T, NG>), dim3(row_grid(g)), dim3(BLOCK),
-                       0, stream, g, (const float4 *)a.part, a.gmax, a.tokens,
-                       a.ignore, a.K, c, 1. / a.temperature, a.logprobs,
-                       a.entropy, a.top_lp, a.top_ids, (float4 *)a.stat);
+static void logprobs_top_join_t(const VocabRows &g, const VocabLogprobs &a,
+                                float c, hipStream_t stream) {
+    hipLaunchKernelGGL((logprobs_top_join<T, NG>), dim3(row_grid(g.rows)),
+                       dim3(BLOCK), 0, stream, g, (const float4 *)a.part,
+                       a.gmax, a.tokens, a.ignore, a.K, c, 1. / a.temperature,
+                       a.logprobs, a.entropy, a.top_lp, a.top_ids,
+                       (float4 *)a.stat);
 }
 
 template <typename T>
@@ -1036,7 +1116,11 @@ static void logprobs_fwd_t(const VocabRows &g, const VocabLogprobs &a,
                            dim3(wave_grid(g)), dim3(BLOCK), 0, stream, g,
                            a.tokens, a.ignore, nullptr, 0, c,
                            (float4 *)a.part, nullptr);
-        logprobs_join_t<T, 0>(g, a, c, stream);
+        hipLaunchKernelGGL((logprobs_join<T>),
+                           dim3(row_grid(CDIV((long)g.rows, WAVES))),
+                           dim3(BLOCK), 0, stream, g, (const float4 *)a.part,
+                           a.tokens, a.ignore, c, 1. / a.temperature,
+                           a.logprobs, a.entropy, (float4 *)a.stat);
         return;
     }
     hipLaunchKernelGGL((vocab_partials<T, true, false, true>),
@@ -1045,10 +1129,10 @@ static void logprobs_fwd_t(const VocabRows &g, const VocabLogprobs &a,
                        a.gmax);
     // maxima per thread; more than VOCAB_MAX_TOP_V tokens are refused before
     const long per = CDIV(CDIV(g.V, (long)GROUP), (long)BLOCK);
-    if (per <= 4) logprobs_join_t<T, 4>(g, a, c, stream);
-    else if (per <= 8) logprobs_join_t<T, 8>(g, a, c, stream);
-    else if (per <= 16) logprobs_join_t<T, 16>(g, a, c, stream);
-    else logprobs_join_t<T, 32>(g, a, c, stream);
+    if (per <= 4) logprobs_top_join_t<T, 4>(g, a, c, stream);
+    else if (per <= 8) logprobs_top_join_t<T, 8>(g, a, c, stream);
+    else if (per <= 16) logprobs_top_join_t<T, 16>(g, a, c, stream);
+    else logprobs_top_join_t<T, 32>(g, a, c, stream);
 }
 
 template <typename T>
@@ -1065,8 +1149,9 @@ static void distill_fwd_t(const VocabRows &g, const VocabDistill &a,
                            dim3(wave_grid(g)), dim3(BLOCK), 0, stream, g,
                            nullptr, 0, nullptr, 0, c, (float4 *)a.part,
                            nullptr);
-    hipLaunchKernelGGL((distill_join<T>), dim3(row_grid(g)), dim3(BLOCK), 0,
-                       stream, g, (const float4 *)a.part, a.teacher_lp, a.ids,
+    hipLaunchKernelGGL((distill_join<T>),
+                       dim3(row_grid(CDIV((long)g.rows, WAVES))), dim3(BLOCK),
+                       0, stream, g, (const float4 *)a.part, a.teacher_lp, a.ids,
                        a.K, a.bucket, c, 1. / a.temperature, a.loss, a.q,
                        (float4 *)a.stat);
 }
