@@ -257,7 +257,7 @@ DEV bool by_product(float mc) { return fabsf(mc) < 0x1p20f; }
 // movement in the operand, then the four rows through scalar registers
 template <int CTRL> DEV float dpp(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(
-        __float_as_int(v), __float_as_int(v), CTRL, 0xf, 0xf, false));
+        0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
 #define DPP_XOR1 0xB1         // quad_perm [1, 0, 3, 2]
 #define DPP_XOR2 0x4E         // quad_perm [2, 3, 0, 1]
@@ -275,8 +275,7 @@ DEV float sum_wave(float v) {
     return (lane_f(v, 0) + lane_f(v, 16)) + (lane_f(v, 32) + lane_f(v, 48));
 }
 template <int CTRL, typename I> DEV I dpp_i(I v) {
-    return (I)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf,
-                                          false);
+    return (I)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
 // over aligned groups of LPG = 8 or 16 lanes
 template <int LPG> DEV int group_max(int v) {
@@ -298,6 +297,13 @@ DEV int max_wave(int v) {
     v = group_max<16>(v);
     return max(max(lane_i(v, 0), lane_i(v, 16)),
                max(lane_i(v, 32), lane_i(v, 48)));
+}
+DEV u32 or_wave(u32 v) {
+    v |= dpp_i<DPP_XOR1>(v);
+    v |= dpp_i<DPP_XOR2>(v);
+    v |= dpp_i<DPP_HALF_MIRROR>(v);
+    v |= dpp_i<DPP_MIRROR>(v);
+    return (u32)(lane_i(v, 0) | lane_i(v, 16) | lane_i(v, 32) | lane_i(v, 48));
 }
 DEV u32 min_wave(u32 v) {
     v = group_min<16>(v);
@@ -332,6 +338,57 @@ DEV float max_wave_f(float v) {
                  fmaxf(lane_f(v, 32), lane_f(v, 48)));
 }
 
+// Each lane's largest pattern of its vector j, over the LPG lanes of a group,
+// to the group's lane j.
+DEV int group_tops(const Vec<float> (&v)[NVEC], int lane) {
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < NVEC; ++j) {
+        Patterns<float> p;
+        v[j].widen(p.hi, p.lo);
+        const int x = group_max<16>(p.top());
+        if (lane % 16 == j) mine = x;
+    }
+    return mine;
+}
+// 16-bit types: two vectors to a register, and at every exchange a lane keeps
+// the half that it is to end with: 15 operations for eight maxima over eight
+// lanes, not 8 * 4.
+template <typename T> DEV int group_tops(const Vec<T> (&v)[NVEC], int lane) {
+    static_assert(NVEC == 8, "eight vectors, eight lanes");
+    s16x2 two[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        Patterns<T> p, q;
+        v[2 * j].widen(p.hi, p.lo);
+        v[2 * j + 1].widen(q.hi, q.lo);
+        const u32 a = __builtin_bit_cast(u32, p.hi);
+        const u32 b = __builtin_bit_cast(u32, q.hi);
+        // low halves of both, high halves of both
+        const u32 lo = __builtin_amdgcn_perm(b, a, 0x05040100);
+        const u32 hi = __builtin_amdgcn_perm(b, a, 0x07060302);
+        two[j] = __builtin_elementwise_max(__builtin_bit_cast(s16x2, lo),
+                                           __builtin_bit_cast(s16x2, hi));
+    }
+    const bool b0 = lane & 1, b1 = lane & 2, b2 = lane & 4;
+    auto exchange = [](s16x2 keep, s16x2 give, auto ctrl) {
+        const u32 o =
+            dpp_i<decltype(ctrl)::value>(__builtin_bit_cast(u32, give));
+        return __builtin_elementwise_max(keep, __builtin_bit_cast(s16x2, o));
+    };
+    // 7 - lane, then lane ^ 2, then lane ^ 1
+    typedef std::integral_constant<int, DPP_HALF_MIRROR> Mirror;
+    typedef std::integral_constant<int, DPP_XOR2> Xor2;
+    typedef std::integral_constant<int, DPP_XOR1> Xor1;
+    const s16x2 p0 = exchange(b2 ? two[2] : two[0], b2 ? two[0] : two[2],
+                              Mirror());
+    const s16x2 p1 = exchange(b2 ? two[3] : two[1], b2 ? two[1] : two[3],
+                              Mirror());
+    const s16x2 q = exchange(b1 ? p1 : p0, b1 ? p0 : p1, Xor2());
+    const s16x2 x = exchange(q, q, Xor1());
+    return b0 ? (int)x.y : (int)x.x;
+}
+
 // ---- partials --------------------------------------------------------------
 // Workgroups go to the 8 XCDs in turn. Giving each XCD a run of consecutive
 // stretches keeps neighbours, which share a cache line where rows are not
@@ -343,11 +400,10 @@ DEV u32 wave_index() {
     return __builtin_amdgcn_readfirstlane(b * WAVES + threadIdx.x / WAVE);
 }
 
-// One wave per stretch. Writes (m, s, t, s_in): m is a reference no smaller
-// than any logit of the stretch; s_in is the part of the sum that belongs to
-// the teacher's entries (EXCL), and s then leaves it out: the rest of the
-// mass is summed, not got as a difference, because a student that has
-// learned leaves little of it. With GRP also the maximum of each GROUP
+// One wave per stretch. Writes (m, s, t, 0). With EXCL the sum leaves out the
+// tokens that a teacher lists (m does not): the rest of the mass is summed,
+// not got as a difference, because a student that has learned leaves little
+// of it. Only vectors that hold such a token look at its bits. With GRP also the maximum of each GROUP
 // consecutive tokens, for the search of the top alternatives.
 //
 // What bounds it: per element one unpacking, one product, one exponential,
@@ -369,32 +425,40 @@ __global__ __launch_bounds__(BLOCK) void vocab_partials(
         if (tokens && tokens[r] == ignore) continue;
         const T *row = row_ptr<T>(g, r);
         const long lo = (long)seg * SEG;
+        // the ids before the stretch: loads arrive in order
+        constexpr int EPL = EXCL ? VOCAB_MAX_K / WAVE : 1;
+        long id[EPL];
+        if (EXCL) {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) {
+                const int k = e * WAVE + lane;
+                id[e] = k < K ? ids[(long)r * K + k] : -1;
+            }
+        }
         Vec<T> v[NVEC];
         load_stretch(row, lo, g.V, lane, v);
+        // the tokens of this stretch that the teacher lists, one bit each
+        u32 hit = 0;  // vectors of the stretch that hold one
         if (EXCL) {
             for (int i = lane; i < SEG / 32; i += WAVE) bits[wid][i] = 0;
             wave_sync();
-            for (int k = lane; k < K; k += WAVE) {
-                const long at = ids[(long)r * K + k] - lo;
-                if (at >= 0 && at < SEG)
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) {
+                const long at = id[e] - lo;
+                if (at >= 0 && at < SEG) {
                     atomicOr(&bits[wid][at >> 5], 1u << (at & 31));
+                    hit |= 1u << ((int)at / (WAVE * N));
+                }
             }
             wave_sync();
+            hit = or_wave(hit);
         }
         // the largest value, by bit patterns; a stretch (or a group) without
         // a value >= 0 is looked at a second time
         int top;
         u32 m_bits;
         if (GRP) {
-            int gm = 0;
-            top = 0;
-#pragma unroll
-            for (int j = 0; j < NVEC; ++j) {
-                Patterns<T> p;
-                v[j].widen(p.hi, p.lo);
-                const int x = group_max<LPG>(p.top());
-                if (lane % LPG == j) gm = x;
-            }
+            const int gm = group_tops(v, lane);
             u32 gbits = (u32)gm;
             const bool mine = lane % LPG < NVEC;
             if (__ballot(mine && gm < 0)) {
@@ -430,15 +494,10 @@ __global__ __launch_bounds__(BLOCK) void vocab_partials(
         }
         const float m = from_pattern<T>(m_bits);
         const float mr = m == -INFINITY ? 0.f : m, mc = mr * c;
-        float s = 0.f, t = 0.f, s_in = 0.f;
+        float s = 0.f, t = 0.f;
         // one vector; the values stay packed until here
         auto sums = [&](const Vec<T> &x, int j, auto diff) {
-            u32 in = 0;
-            if (EXCL) {
-                const int at = (j * WAVE + lane) * N;
-                in = (bits[wid][at >> 5] >> (at & 31)) & ((1u << N) - 1);
-            }
-            if (!EXCL || __ballot(in != 0) == 0) {
+            if (!EXCL || !(hit >> j & 1)) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const float d = diff(x.get(i)), e = exp2_hw(d);
@@ -448,12 +507,14 @@ __global__ __launch_bounds__(BLOCK) void vocab_partials(
                     if (ENT) t = fmaf(fmaxf(d, -300.f), e, t);
                 }
             } else {
+                const int at = (j * WAVE + lane) * N;
+                const u32 in = bits[wid][at >> 5] >> (at & 31);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const float e = exp2_hw(diff(x.get(i)));
-                    const bool listed = in >> i & 1;
-                    s += listed ? 0.f : e;
-                    s_in += listed ? e : 0.f;
+                    const u32 e = __float_as_uint(exp2_hw(diff(x.get(i))));
+                    // all ones where listed
+                    const u32 mask = (u32)((int)(in << (31 - i)) >> 31);
+                    s += __uint_as_float(e & ~mask);
                 }
             }
         };
@@ -470,15 +531,14 @@ __global__ __launch_bounds__(BLOCK) void vocab_partials(
         }
         s = sum_wave(s);
         if (ENT) t = sum_wave(t);
-        if (EXCL) s_in = sum_wave(s_in);
-        if (lane == 0) part[w] = make_float4(m, s, t, s_in);
+        if (lane == 0) part[w] = make_float4(m, s, t, 0.f);
     }
 }
 
 // ---- join ------------------------------------------------------------------
 struct RowStat {
     float m;           // largest logit, 0 where there is none
-    double s, t, s_in; // against m*c itself
+    double s, t;       // against m*c itself
     double delta;      // m*c less its rounded value: 2^(x*c - mc) is
                        // 2^delta times too large
 };
@@ -493,7 +553,7 @@ DEV RowStat join_parts(const float4 *p, int nseg, float c, int lane) {
     const float mc = st.m * c;
     const double exact = (double)st.m * c;
     st.delta = by_product(mc) ? exact - mc : 0.;
-    double s = 0, t = 0, s_in = 0;
+    double s = 0, t = 0;
     for (int i = lane; i < nseg; i += WAVE) {
         const float4 q = p[i];
         const float qm = q.x == -INFINITY ? 0.f : q.x;
@@ -504,11 +564,9 @@ DEV RowStat join_parts(const float4 *p, int nseg, float c, int lane) {
         if (q.x == -INFINITY || d < -300) d = -300;
         const double f = exp2(d);
         s += q.y * f;
-        s_in += q.w * f;
-        t += (q.z + d * ((double)q.y + q.w)) * f;
+        t += (q.z + d * q.y) * f;
     }
     st.s = sum_wave_d(s);
-    st.s_in = sum_wave_d(s_in);
     st.t = sum_wave_d(t);
     return st;
 }
@@ -824,6 +882,8 @@ __global__ __launch_bounds__(BLOCK) void distill_join(
     int bucket, float c, double inv_t, float *__restrict__ loss,
     float *__restrict__ q_out, float4 *__restrict__ stat) {
     constexpr int EPL = VOCAB_MAX_K / WAVE;
+    constexpr int HASH = 2 * VOCAB_MAX_K;  // never more than half full
+    __shared__ int seen[WAVES][HASH];
     const int lane = threadIdx.x % WAVE;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     for (u32 r = blockIdx.x * WAVES + wid; r < (u32)g.rows;
@@ -880,7 +940,24 @@ __global__ __launch_bounds__(BLOCK) void distill_join(
             continue;
         }
         const RowStat st = join_parts(part + (long)r * g.nseg, g.nseg, c, lane);
-        const double s = st.s + st.s_in;
+        double s = st.s;
+        if (bucket) {
+            // the listed tokens' part, each token once
+            for (int i = lane; i < HASH; i += WAVE) seen[wid][i] = -1;
+            wave_sync();
+            double s_in = 0.;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e)
+                if (id[e] >= 0 && id[e] < g.V) {
+                    u32 at = ((u32)id[e] * 2654435761u) / (~0u / HASH + 1);
+                    int old;
+                    while ((old = atomicCAS(&seen[wid][at], -1, (int)id[e])) !=
+                               -1 && old != (int)id[e])
+                        at = (at + 1) % HASH;
+                    if (old == -1) s_in += exp2(((double)x[e] - st.m) * c);
+                }
+            s += sum_wave_d(s_in);
+        }
         const bool none = s == 0, bad = !(s < INFINITY);
         const double ln_s = log(s);
         double sum = 0.;
