@@ -434,7 +434,7 @@ torch::Tensor token_logprobs_bwd(
         CHECK_ROWS(*d_top, torch::kFloat32, g.rows * K);
         a.d_top = d_top->data_ptr<float>();
     }
-    a.stat = (const float4 *)stat.data_ptr<float>();
+    a.stat = stat.data_ptr<float>();
     a.c = (float)(1.4426950408889634 / temperature);
     a.inv_t = (float)(1. / temperature);
     a.K = (int)K;
@@ -449,7 +449,7 @@ torch::Tensor token_logprobs_bwd(
     return out;
 }
 
-// -> loss, q, stat
+// -> loss, entry, stat
 std::vector<torch::Tensor> topk_distillation_fwd(torch::Tensor logits,
                                                  torch::Tensor teacher_logprobs,
                                                  torch::Tensor teacher_ids,
@@ -464,7 +464,7 @@ std::vector<torch::Tensor> topk_distillation_fwd(torch::Tensor logits,
     CHECK_ROWS(teacher_logprobs, torch::kFloat32, g.rows * K);
     const auto f32 = logits.options().dtype(torch::kFloat32);
     auto loss = torch::empty(lead_sizes(logits), f32);
-    auto q = torch::empty({g.rows, K}, f32);
+    auto entry = torch::empty({g.rows, K, 2}, f32.dtype(torch::kInt32));
     auto stat = torch::empty({g.rows, 4}, f32);
     if (g.rows > 0) {
         auto part = torch::empty({g.rows, g.nseg, 4}, f32);
@@ -476,33 +476,32 @@ std::vector<torch::Tensor> topk_distillation_fwd(torch::Tensor logits,
         a.temperature = temperature;
         a.part = part.data_ptr<float>();
         a.loss = loss.data_ptr<float>();
-        a.q = q.data_ptr<float>();
+        a.entry = entry.data_ptr<int>();
         a.stat = stat.data_ptr<float>();
         distill_fwd_launch(&g, &a, vocab_dtype(logits), cur_stream());
         C10_HIP_KERNEL_LAUNCH_CHECK();
     }
-    return {loss, q, stat};
+    return {loss, entry, stat};
 }
 
 torch::Tensor topk_distillation_bwd(torch::Tensor dloss, torch::Tensor logits,
-                                    torch::Tensor teacher_ids, torch::Tensor q,
-                                    torch::Tensor stat, double temperature) {
+                                    torch::Tensor entry, torch::Tensor stat,
+                                    double temperature) {
     c10::OptionalDeviceGuard guard(logits.device());
     VocabRows g = vocab_rows_or_copy(logits);
-    const int64_t K = teacher_ids.size(-1);
+    TORCH_CHECK(entry.dim() == 3, "entry must be [rows, K, 2]");
+    const int64_t K = entry.size(1);
     TORCH_CHECK(K >= 1 && K <= VOCAB_MAX_K, "entries per row");
     CHECK_ROWS(dloss, torch::kFloat32, g.rows);
-    CHECK_ROWS(teacher_ids, torch::kInt64, g.rows * K);
-    CHECK_ROWS(q, torch::kFloat32, g.rows * K);
+    CHECK_ROWS(entry, torch::kInt32, g.rows * K * 2);
     CHECK_ROWS(stat, torch::kFloat32, g.rows * 4ll);
     VocabGrad a = {};
-    a.stat = (const float4 *)stat.data_ptr<float>();
+    a.stat = stat.data_ptr<float>();
     a.c = (float)(1.4426950408889634 / temperature);
     a.inv_t = (float)(1. / temperature);
     a.K = (int)K;
     a.d_row = dloss.data_ptr<float>();
-    a.q = q.data_ptr<float>();
-    a.ids = teacher_ids.data_ptr<int64_t>();
+    a.entry = entry.data_ptr<int>();
     auto out = torch::empty(logits.sizes(), logits.options());
     if (g.rows > 0) {
         vocab_grad_launch(&g, &a, 1, out.data_ptr(), vocab_dtype(logits),

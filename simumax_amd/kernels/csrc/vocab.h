@@ -35,18 +35,19 @@ struct VocabDistill {
     const long *ids;          // [rows, K]
     int K, bucket;
     double temperature;
-    float *part, *loss, *q, *stat;
+    float *part, *loss, *stat;
+    int *entry;  // [rows, K, 2]: id or -1, and the weight's bits
 };
 
 struct VocabGrad {
-    const float4 *stat;
+    const float *stat;  // [rows, 4]
     float c, inv_t;
-    int K;
     const float *d_row;      // of the log probabilities, or of the loss
     const float *d_entropy;  // null where none
     const float *d_top;      // [rows, K], null where none
-    const float *q;          // [rows, K], the teacher's weights
+    const int *entry;        // [rows, K, 2], the teacher's
     const long *ids;         // [rows, K]
-    const long *tokens;      // [rows] or null
+    int K;
+    const long *tokens;  // [rows] or null
     long ignore;
 };

@@ -30,6 +30,7 @@
 #define BLOCK 256
 #define WAVES (BLOCK / WAVE)
 #define NVEC 8    // 16-byte vectors per lane and stretch
+#define NGRAD 4   // the same in the gradient
 #define GROUP 64  // tokens per maximum kept for the top alternatives
 #define CAP 512   // candidates for them that are ranked at once
 
@@ -62,6 +63,15 @@ template <typename T> struct Vec {
     }
     DEV float get(int i) const;
     DEV void put(int i, float a, float b);  // elements i and i + 1, i even
+    DEV float pick(int i) const {  // get, where i differs between lanes
+        constexpr int PER = N / 4;
+        const int k = i / PER;
+        const u32 a = k & 1 ? w[1] : w[0], b = k & 1 ? w[3] : w[2];
+        Vec<T> one;
+        one.w[0] = k & 2 ? b : a;
+        if constexpr (PER == 2) one.w[0] >>= (i & 1) * 16;
+        return one.get(0);
+    }
     // Largest and smallest bit pattern, as signed and unsigned numbers: of
     // floats of which one at least is not negative the first is the largest
     // float, of negative floats the second is. Packed, a half operation per
@@ -182,31 +192,31 @@ template <typename T> DEV Vec<T> load_vec(const T *row, long at, long V) {
 }
 
 // a wave's stretch of a row; only a row's last one can be cut short
-template <typename T>
+template <typename T, int NV>
 DEV void load_stretch(const T *row, long lo, long V, int lane,
-                      Vec<T> (&v)[NVEC]) {
+                      Vec<T> (&v)[NV]) {
     constexpr int N = Vec<T>::N;
-    constexpr int SEG = WAVE * NVEC * N;
+    constexpr int SEG = WAVE * NV * N;
     if (lo + SEG <= V) {
         const T *p = row + lo + lane * N;
 #pragma unroll
-        for (int j = 0; j < NVEC; ++j) v[j].stream_in(p + j * WAVE * N);
+        for (int j = 0; j < NV; ++j) v[j].stream_in(p + j * WAVE * N);
     } else if (V >= N) {
         const int rest = (int)(V - lo);  // below SEG
 #pragma unroll
-        for (int j = 0; j < NVEC; ++j) {
+        for (int j = 0; j < NV; ++j) {
             const int at = (j * WAVE + lane) * N;
             v[j].load(row + lo + min(at, rest - N));
         }
 #pragma unroll
-        for (int j = 0; j < NVEC; ++j) {
+        for (int j = 0; j < NV; ++j) {
             const int at = (j * WAVE + lane) * N;
             shift_in_pad(v[j], min(max(at + N - rest, 0), N));
         }
     } else {
         v[0] = load_vec(row, (long)lane * N, V);
 #pragma unroll
-        for (int j = 1; j < NVEC; ++j) v[j].w = pad_word<T>();
+        for (int j = 1; j < NV; ++j) v[j].w = pad_word<T>();
     }
 }
 
@@ -410,7 +420,7 @@ DEV u32 wave_index() {
 // one or two sums and half an operation for the maximum, beside 2 or 4 bytes.
 template <typename T, bool ENT, bool EXCL, bool GRP>
 __global__ __launch_bounds__(BLOCK) void vocab_partials(
-    VocabRows g, const long *__restrict__ tokens, long ignore,
+    VocabRows g, u32 first, const long *__restrict__ tokens, long ignore,
     const long *__restrict__ ids, int K, float c, float4 *__restrict__ part,
     float *__restrict__ gmax) {
     constexpr int N = Vec<T>::N;
@@ -419,123 +429,152 @@ __global__ __launch_bounds__(BLOCK) void vocab_partials(
     __shared__ u32 bits[EXCL ? WAVES : 1][EXCL ? SEG / 32 : 1];
     const int lane = threadIdx.x % WAVE;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    const u32 total = (u32)g.rows * g.nseg;  // below 2^31, as is w's step
-    for (u32 w = wave_index(); w < total; w += gridDim.x * WAVES) {
-        const int r = w / (u32)g.nseg, seg = w - (u32)r * g.nseg;
-        if (tokens && tokens[r] == ignore) continue;
-        const T *row = row_ptr<T>(g, r);
-        const long lo = (long)seg * SEG;
-        // the ids before the stretch: loads arrive in order
-        constexpr int EPL = EXCL ? VOCAB_MAX_K / WAVE : 1;
-        long id[EPL];
-        if (EXCL) {
+    const u32 w = first + wave_index();  // below 2^32
+    if (w >= (u32)g.rows * g.nseg) return;
+    const int r = w / (u32)g.nseg, seg = w - (u32)r * g.nseg;
+    if (tokens && tokens[r] == ignore) return;
+    const T *row = row_ptr<T>(g, r);
+    const long lo = (long)seg * SEG;
+    // the ids before the stretch: loads arrive in order
+    constexpr int EPL = EXCL ? VOCAB_MAX_K / WAVE : 1;
+    long id[EPL];
+    if (EXCL) {
 #pragma unroll
-            for (int e = 0; e < EPL; ++e) {
-                const int k = e * WAVE + lane;
-                id[e] = k < K ? ids[(long)r * K + k] : -1;
-            }
+        for (int e = 0; e < EPL; ++e) {
+            const int k = e * WAVE + lane;
+            id[e] = k < K ? ids[(long)r * K + k] : -1;
         }
-        Vec<T> v[NVEC];
-        load_stretch(row, lo, g.V, lane, v);
-        // the tokens of this stretch that the teacher lists, one bit each
-        u32 hit = 0;  // vectors of the stretch that hold one
-        if (EXCL) {
-            for (int i = lane; i < SEG / 32; i += WAVE) bits[wid][i] = 0;
-            wave_sync();
-#pragma unroll
-            for (int e = 0; e < EPL; ++e) {
-                const long at = id[e] - lo;
-                if (at >= 0 && at < SEG) {
-                    atomicOr(&bits[wid][at >> 5], 1u << (at & 31));
-                    hit |= 1u << ((int)at / (WAVE * N));
-                }
-            }
-            wave_sync();
-            hit = or_wave(hit);
-        }
-        // the largest value, by bit patterns; a stretch (or a group) without
-        // a value >= 0 is looked at a second time
-        int top;
-        u32 m_bits;
-        if (GRP) {
-            const int gm = group_tops(v, lane);
-            u32 gbits = (u32)gm;
-            const bool mine = lane % LPG < NVEC;
-            if (__ballot(mine && gm < 0)) {
-#pragma unroll
-                for (int j = 0; j < NVEC; ++j) {
-                    Patterns<T> p;
-                    v[j].widen(p.hi, p.lo);
-                    const u32 x = group_min<LPG>(p.bottom());
-                    if (lane % LPG == j && gm < 0) gbits = x;
-                }
-            }
-            if (mine) {
-                // lane (group q of a vector, j) has group j * (64 / LPG) + q
-                const int q = lane / LPG, j = lane % LPG;
-                gmax[(long)w * (SEG / GROUP) + j * (WAVE / LPG) + q] =
-                    from_pattern<T>(gbits);
-            }
-            top = max_wave(mine ? gm : -2147483647 - 1);
-            m_bits = (u32)top;
-            if (top < 0) m_bits = min_wave(mine ? gbits : 0xffffffffu);
-        } else {
-            Patterns<T> p;
-#pragma unroll
-            for (int j = 0; j < NVEC; ++j) v[j].widen(p.hi, p.lo);
-            top = max_wave(p.top());
-            m_bits = (u32)top;
-            if (top < 0) {
-                Patterns<T> n;
-#pragma unroll
-                for (int j = 0; j < NVEC; ++j) v[j].widen(n.hi, n.lo);
-                m_bits = min_wave(n.bottom());
-            }
-        }
-        const float m = from_pattern<T>(m_bits);
-        const float mr = m == -INFINITY ? 0.f : m, mc = mr * c;
-        float s = 0.f, t = 0.f;
-        // one vector; the values stay packed until here
-        auto sums = [&](const Vec<T> &x, int j, auto diff) {
-            if (!EXCL || !(hit >> j & 1)) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float d = diff(x.get(i)), e = exp2_hw(d);
-                    s += e;
-                    // 2^-300 is 0, and (-inf) * 0 would be NaN; NaN is in e
-                    // already
-                    if (ENT) t = fmaf(fmaxf(d, -300.f), e, t);
-                }
-            } else {
-                const int at = (j * WAVE + lane) * N;
-                const u32 in = bits[wid][at >> 5] >> (at & 31);
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const u32 e = __float_as_uint(exp2_hw(diff(x.get(i))));
-                    // all ones where listed
-                    const u32 mask = (u32)((int)(in << (31 - i)) >> 31);
-                    s += __uint_as_float(e & ~mask);
-                }
-            }
-        };
-        if (by_product(mc)) {
-#pragma unroll
-            for (int j = 0; j < NVEC; ++j)
-                sums(v[j], j, [&](float x) { return fmaf(x, c, -mc); });
-        } else {
-            // rare: read again, one vector at a time, rather than held twice
-#pragma unroll 1
-            for (int j = 0; j < NVEC; ++j)
-                sums(load_vec(row, lo + (long)(j * WAVE + lane) * N, g.V), j,
-                     [&](float x) { return (x - mr) * c; });
-        }
-        s = sum_wave(s);
-        if (ENT) t = sum_wave(t);
-        if (lane == 0) part[w] = make_float4(m, s, t, 0.f);
     }
+    Vec<T> v[NVEC];
+    load_stretch(row, lo, g.V, lane, v);
+    // the tokens of this stretch that the teacher lists, one bit each
+    u32 hit = 0;  // vectors of the stretch that hold one
+    if (EXCL) {
+        for (int i = lane; i < SEG / 32; i += WAVE) bits[wid][i] = 0;
+        wave_sync();
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            const long at = id[e] - lo;
+            if (at >= 0 && at < SEG) {
+                atomicOr(&bits[wid][at >> 5], 1u << (at & 31));
+                hit |= 1u << ((int)at / (WAVE * N));
+            }
+        }
+        wave_sync();
+        hit = or_wave(hit);
+    }
+    // the largest value, by bit patterns; a stretch (or a group) without
+    // a value >= 0 is looked at a second time
+    int top;
+    u32 m_bits;
+    if (GRP) {
+        const int gm = group_tops(v, lane);
+        u32 gbits = (u32)gm;
+        const bool mine = lane % LPG < NVEC;
+        if (__ballot(mine && gm < 0)) {
+#pragma unroll
+            for (int j = 0; j < NVEC; ++j) {
+                Patterns<T> p;
+                v[j].widen(p.hi, p.lo);
+                const u32 x = group_min<LPG>(p.bottom());
+                if (lane % LPG == j && gm < 0) gbits = x;
+            }
+        }
+        if (mine) {
+            // lane (group q of a vector, j) has group j * (64 / LPG) + q
+            const int q = lane / LPG, j = lane % LPG;
+            gmax[(long)w * (SEG / GROUP) + j * (WAVE / LPG) + q] =
+                from_pattern<T>(gbits);
+        }
+        top = max_wave(mine ? gm : -2147483647 - 1);
+        m_bits = (u32)top;
+        if (top < 0) m_bits = min_wave(mine ? gbits : 0xffffffffu);
+    } else {
+        Patterns<T> p;
+#pragma unroll
+        for (int j = 0; j < NVEC; ++j) v[j].widen(p.hi, p.lo);
+        top = max_wave(p.top());
+        m_bits = (u32)top;
+        if (top < 0) {
+            Patterns<T> n;
+#pragma unroll
+            for (int j = 0; j < NVEC; ++j) v[j].widen(n.hi, n.lo);
+            m_bits = min_wave(n.bottom());
+        }
+    }
+    const float m = from_pattern<T>(m_bits);
+    const float mr = m == -INFINITY ? 0.f : m, mc = mr * c;
+    float s = 0.f, t = 0.f;
+    // one vector; the values stay packed until here
+    auto sums = [&](const Vec<T> &x, int j, auto diff) {
+        if (!EXCL || !(hit >> j & 1)) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float d = diff(x.get(i)), e = exp2_hw(d);
+                s += e;
+                // 2^-300 is 0, and (-inf) * 0 would be NaN; NaN is in e
+                // already
+                if (ENT) t = fmaf(fmaxf(d, -300.f), e, t);
+            }
+        } else {
+            const int at = (j * WAVE + lane) * N;
+            const u32 in = bits[wid][at >> 5] >> (at & 31);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const u32 e = __float_as_uint(exp2_hw(diff(x.get(i))));
+                // all ones where listed
+                const u32 mask = (u32)((int)(in << (31 - i)) >> 31);
+                s += __uint_as_float(e & ~mask);
+            }
+        }
+    };
+    if (by_product(mc)) {
+#pragma unroll
+        for (int j = 0; j < NVEC; ++j)
+            sums(v[j], j, [&](float x) { return fmaf(x, c, -mc); });
+    } else {
+        // rare: read again, one vector at a time, rather than held twice
+#pragma unroll 1
+        for (int j = 0; j < NVEC; ++j)
+            sums(load_vec(row, lo + (long)(j * WAVE + lane) * N, g.V), j,
+                 [&](float x) { return (x - mr) * c; });
+    }
+    s = sum_wave(s);
+    if (ENT) t = sum_wave(t);
+    if (lane == 0) part[w] = make_float4(m, s, t, 0.f);
 }
 
 // ---- join ------------------------------------------------------------------
+// 2^d and ln v in 64 bits, small: the library's take 60 registers more in
+// kernels that live from their occupancy. 2^d by the power series of e^x for
+// |x| <= ln 2 / 2, whose next term is below 2^-53; NaN stays NaN.
+DEV double exp2_d(double d) {
+    d = d < -2000. ? -2000. : d;
+    const double i = rint(d), x = (d - i) * 0.6931471805599453;
+    double p = 1. / 6227020800.;  // 1 / 13!
+    p = fma(p, x, 1. / 479001600.);
+    p = fma(p, x, 1. / 39916800.);
+    p = fma(p, x, 1. / 3628800.);
+    p = fma(p, x, 1. / 362880.);
+    p = fma(p, x, 1. / 40320.);
+    p = fma(p, x, 1. / 5040.);
+    p = fma(p, x, 1. / 720.);
+    p = fma(p, x, 1. / 120.);
+    p = fma(p, x, 1. / 24.);
+    p = fma(p, x, 1. / 6.);
+    p = fma(p, x, 0.5);
+    p = fma(p, x, 1.);
+    p = fma(p, x, 1.);
+    return __builtin_ldexp(p, (int)i);
+}
+// the 32-bit logarithm, and what it leaves over: for r = v / 2^y - 1, below
+// 2^-18, ln v = y ln 2 + r - r^2 / 2 + r^3 / 3. For normal 32-bit v.
+DEV double log_d(double v) {
+    const double y = __builtin_amdgcn_logf((float)v);
+    const double r = fma(v, exp2_d(-y), -1.);
+    return fma(y, 0.6931471805599453, r - r * r * (0.5 - r * (1. / 3.)));
+}
+
 struct RowStat {
     float m;           // largest logit, 0 where there is none
     double s, t;       // against m*c itself
@@ -544,9 +583,13 @@ struct RowStat {
 };
 
 // one wave joins a row's stretches, each lane's in order, in 64 bits
-DEV RowStat join_parts(const float4 *p, int nseg, float c, int lane) {
-    float m = -INFINITY;
-    for (int i = lane; i < nseg; i += WAVE) m = fmaxf(m, p[i].x);
+DEV float4 first_part(const float4 *p, int nseg, int lane) {
+    return lane < nseg ? p[lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+}
+DEV RowStat join_parts(float4 first, const float4 *p, int nseg, float c,
+                       int lane) {
+    float m = first.x;
+    for (int i = lane + WAVE; i < nseg; i += WAVE) m = fmaxf(m, p[i].x);
     m = max_wave_f(m);
     RowStat st;
     st.m = m == -INFINITY ? 0.f : m;
@@ -554,15 +597,15 @@ DEV RowStat join_parts(const float4 *p, int nseg, float c, int lane) {
     const double exact = (double)st.m * c;
     st.delta = by_product(mc) ? exact - mc : 0.;
     double s = 0, t = 0;
-    for (int i = lane; i < nseg; i += WAVE) {
-        const float4 q = p[i];
+    for (int i = lane; i < max(nseg, WAVE); i += WAVE) {
+        const float4 q = i == lane ? first : i < nseg ? p[i] : first_part(p, 0, 0);
         const float qm = q.x == -INFINITY ? 0.f : q.x;
         // against each stretch's own rounded reference, where there is one
         const float qc = qm * c;
         double d = (by_product(qc) ? (double)qc : (double)qm * c) - exact;
         // adds nothing, but NaN stays NaN
         if (q.x == -INFINITY || d < -300) d = -300;
-        const double f = exp2(d);
+        const double f = exp2_d(d);
         s += q.y * f;
         t += (q.z + d * q.y) * f;
     }
@@ -582,92 +625,176 @@ template <typename T> struct Order {
         const u32 b = __float_as_uint(x + 0.f);
         return (b & 0x80000000u ? ~b : b | 0x80000000u) >> LOW;
     }
+    static DEV float value(u32 order) {
+        const u32 b = order << LOW;
+        return __uint_as_float(b & 0x80000000u ? b ^ 0x80000000u
+                                               : ~(b | ((1u << LOW) - 1)));
+    }
 };
+
+#define GROUPS (VOCAB_MAX_K + VOCAB_MAX_K / 2)  // groups looked into at most
+
+#define BINS (4 * BLOCK)
 
 struct TopShared {
-    u64 key[CAP];               // (order, ~index) of the candidates
-    int group[VOCAB_MAX_K];     // groups that can hold alternatives
-    int count[2][WAVES];        // of block_count, two turns
+    u64 key[CAP];              // (order, ~index) of the candidates
+    int group[GROUPS];         // groups that can hold alternatives
+    u32 bin[BINS];             // counts of maxima
+    int4 count[2][WAVES];      // of block_count, two turns
     int ties[32 * WAVES];
-    int n_group, n_key;
+    u32 top[WAVES];
+    int total[WAVES];
+    u32 bound;
+    int n_group, n_key, reach;
 };
 
-// number of true predicates in the workgroup, given each wave's own. `turn`
+// sums over the workgroup of three numbers that each wave has. `turn`
 // alternates between calls, so one barrier is enough.
-DEV int block_count(int wave_count, TopShared &sh, int &turn) {
-    if (threadIdx.x % WAVE == 0) sh.count[turn][threadIdx.x / WAVE] = wave_count;
+DEV int3 block_count(int a, int b, int c, TopShared &sh, int &turn) {
+    if (threadIdx.x % WAVE == 0)
+        sh.count[turn][threadIdx.x / WAVE] = make_int4(a, b, c, 0);
     __syncthreads();
-    int n = 0;
+    int3 n = make_int3(0, 0, 0);
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) n += sh.count[turn][w];
+    for (int w = 0; w < WAVES; ++w) {
+        const int4 o = sh.count[turn][w];
+        n.x += o.x;
+        n.y += o.y;
+        n.z += o.z;
+    }
     turn ^= 1;
     return n;
 }
 
-// calls f(order, index, valid) for every token of the chosen groups; all
-// lanes take part in every call
-template <typename T, typename F>
-DEV void for_candidates(const T *row, long V, const TopShared &sh, int groups,
-                        F f) {
-    constexpr int N = Vec<T>::N, LPG = GROUP / N;
-    for (int i = 0; i < groups * LPG; i += BLOCK) {
-        const int slot = i + threadIdx.x;
-        const bool on = slot < groups * LPG;
-        const long at =
-            on ? (long)sh.group[slot / LPG] * GROUP + slot % LPG * N : V;
-        const Vec<T> v = load_vec(row, at, V);
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-            f(Order<T>::of(v.get(k)), (u32)(at + k), at + k < V);
+// The largest bound, by `bits` bits from the top, that at least `least` keys
+// reach, two bits a turn; stops early where no more than `most` reach it.
+// counter(b) gives a wave's number of keys >= b. `reach` starts with how many
+// reach 0 and ends with how many reach the bound.
+template <typename F>
+DEV u32 search_bound(int bits, int least, int most, int &reach, TopShared &sh,
+                     int &turn, F counter) {
+    u32 bound = 0;
+#pragma unroll 1
+    for (int shift = (bits - 1) & ~1; shift >= 0; shift -= 2) {
+        // of an odd number of bits the first turn has only one
+        const bool two = shift + 1 < bits;
+        const int a = counter(bound + (1u << shift));
+        const int b = two ? counter(bound + (2u << shift)) : 0;
+        const int c = two ? counter(bound + (3u << shift)) : 0;
+        const int3 n = block_count(a, b, c, sh, turn);
+        const int step = n.z >= least ? 3 : n.y >= least ? 2
+                         : n.x >= least                  ? 1 : 0;
+        bound += (u32)step << shift;
+        reach = step == 3 ? n.z : step == 2 ? n.y : step == 1 ? n.x : reach;
+        if (reach <= most) break;
     }
+    return bound;
+}
+
+// inclusive sum over the lanes up to this one
+DEV int scan_wave(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    // the last lane of each row of 16 to the next, of each half to the next
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
+// The same bound for the groups' maxima, from one count of how far each is
+// below the largest, in steps of a bfloat16 (eight octaves: BINS = 1024).
+// False where fewer than K are that near, or where the step's maxima are
+// more than `most` and the type has finer ones.
+template <typename T, int NG>
+DEV bool bound_by_bins(const u32 (&key)[NG], int K, int most, u32 &bound,
+                       int &reach, TopShared &sh) {
+    constexpr int FINE = 16 - Order<T>::LOW;
+    const int tid = threadIdx.x, lane = tid % WAVE, wid = tid / WAVE;
+    u32 top = 0;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) top = max(top, key[i]);
+    top >>= FINE;  // maxima are below 2^31 now: signed comparison serves
+    top = (u32)max_wave((int)top);
+    if (lane == 0) sh.top[wid] = top;
+    *(int4 *)&sh.bin[tid * 4] = make_int4(0, 0, 0, 0);
+    if (tid == 0) sh.reach = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = max(top, sh.top[w]);
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        const u32 below = top - (key[i] >> FINE);
+        if (key[i] && below < BINS) atomicAdd(&sh.bin[below], 1u);
+    }
+    __syncthreads();
+    const int4 b = *(const int4 *)&sh.bin[tid * 4];
+    const int own = b.x + b.y + b.z + b.w, upto = scan_wave(own);
+    if (lane == WAVE - 1) sh.total[wid] = upto;
+    __syncthreads();
+    int before = upto - own;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+        if (w < wid) before += sh.total[w];
+    if (before < K && before + own >= K) {
+        // the K-th is one of this thread's four
+        int n = before + b.x, at = 0;
+        if (n < K) { n += b.y; at = 1; }
+        if (n < K) { n += b.z; at = 2; }
+        if (n < K) { n += b.w; at = 3; }
+        sh.bound = (top - (tid * 4 + at)) << FINE;
+        sh.reach = n;
+    }
+    __syncthreads();
+    bound = sh.bound;
+    reach = sh.reach;
+    return reach > 0 && (FINE == 0 || reach <= most);
 }
 
 // The K largest of a row, (value down, index up), from its groups' maxima.
 // The K groups of the largest (maximum, lowest index) hold them all: each of
-// these has a token at least as good as any token of the others. The K-th
-// maximum is found by bits; tokens of those groups that reach it are the
+// these has a token at least as good as any token of the others. So a bound
+// is searched that between K and 3/2 K (or 16 more) groups reach, or, where
+// maxima are equal, exactly the K-th one, and then the first groups of those
+// that equal it. Tokens of these groups that reach the bound are the
 // candidates, hardly more than K in a row without structure; each one's rank
 // is the number of better ones. Where more than CAP reach it (groups with
 // many large tokens, or a vocabulary of few groups), a higher bound is
 // searched among the tokens themselves, and, where one value alone has too
 // many, a bound on the index. The whole takes NG maxima per thread.
-template <typename T, int NG>
-DEV void top_alternatives(const T *row, long V, const float *gmax, int K,
-                          TopShared &sh, float *top_lp, long *top_ids,
-                          double m, double inv_t, double ln_s, bool none) {
+//
+// What bounds it is latency: barriers, and the groups' loads. `meanwhile` is
+// work of the caller's that goes between those loads and their use.
+template <typename T, int NG, typename F>
+DEV void top_alternatives(const T *row, long g_V, const u32 (&key)[NG], int K,
+                          TopShared &sh, F meanwhile, float *top_lp,
+                          long *top_ids) {
+    constexpr int N = Vec<T>::N, LPG = GROUP / N;
+    constexpr int AHEAD = 4;  // vectors per thread in flight
     const int tid = threadIdx.x, lane = tid % WAVE, wid = tid / WAVE;
-    const int G = (int)((V + GROUP - 1) / GROUP);
+    const int G = (int)((g_V + GROUP - 1) / GROUP);
     int turn = 0;
     if (tid == 0) sh.n_group = sh.n_key = 0;
-    u32 key[NG];
+    u32 bound = Order<T>::of(-INFINITY);  // 0 are keys of no group
+    int reach = G;  // how many groups reach it
+    const int most = min(K + max(K / 2, 16), GROUPS);
+    if (G <= most) {
+        __syncthreads();  // n_group, n_key
+    } else if (!bound_by_bins<T, NG>(key, K, most, bound, reach, sh)) {
+        reach = G;
+        bound = search_bound(Order<T>::BITS, K, most, reach, sh, turn,
+                             [&](u32 b) {
+                                 int n = 0;
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-        const int g = i * BLOCK + tid;
-        key[i] = g < G ? Order<T>::of(gmax[g]) : 0;
+                                 for (int i = 0; i < NG; ++i)
+                                     n += __popcll(__ballot(key[i] >= b));
+                                 return n;
+                             });
     }
-    u32 bound = 0;  // the K-th largest maximum, all bits below it 0
-    int reach = G;  // how many reach it
-    int KG = K;
-    if (G <= K) {
-        bound = 1;
-        KG = G;
-    } else {
-        for (int bit = Order<T>::BITS - 1; bit >= 0; --bit) {
-            const u32 b = bound | 1u << bit;
-            int n = 0;
-#pragma unroll
-            for (int i = 0; i < NG; ++i) n += __popcll(__ballot(key[i] >= b));
-            n = block_count(n, sh, turn);
-            if (n >= K) {
-                bound = b;
-                reach = n;
-                if (n == K) break;
-            }
-        }
-    }
-    // of the groups that equal the bound, those of lowest index
-    int before[NG], quota = BLOCK * NG;
-    if (reach > KG) {
+    if (reach > most) {
+        // `bound` is the K-th maximum: of the groups that equal it, those of
+        // lowest index
         int above = 0;
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
@@ -675,93 +802,161 @@ DEV void top_alternatives(const T *row, long V, const float *gmax, int K,
             const int ties = __popcll(__ballot(key[i] == bound));
             if (lane == 0) sh.ties[i * WAVES + wid] = ties;
         }
-        quota = KG - block_count(above, sh, turn);
-        int run = 0;
+        const int quota = K - block_count(above, 0, 0, sh, turn).x;
+        // how many such groups come before each wave's i-th 64
+        if (wid == 0) {
+            int run = 0;
 #pragma unroll
-        for (int i = 0; i < NG; ++i)
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                if (w == wid) before[i] = run;
-                run += sh.ties[i * WAVES + w];
+            for (int i = 0; i < NG * WAVES; i += WAVE) {
+                const bool on = i + lane < NG * WAVES;
+                const int own = on ? sh.ties[i + lane] : 0;
+                const int upto = scan_wave(own);
+                if (on) sh.ties[i + lane] = run + upto - own;
+                run += lane_i(upto, WAVE - 1);
             }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const u64 ties = __ballot(key[i] == bound);
+            const int nth = sh.ties[i * WAVES + wid] +
+                            __popcll(ties & ((1ull << lane) - 1));
+            if (key[i] > bound || (key[i] == bound && nth < quota))
+                sh.group[atomicAdd(&sh.n_group, 1)] = i * BLOCK + tid;
+        }
+        reach = K;
     } else {
-        __syncthreads();  // n_group, n_key
+        int own = 0;
 #pragma unroll
-        for (int i = 0; i < NG; ++i) before[i] = 0;
-    }
+        for (int i = 0; i < NG; ++i) own += key[i] >= bound;
+        if (own) {
+            int slot = atomicAdd(&sh.n_group, own);
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-        const u64 ties = __ballot(key[i] == bound);
-        const int nth = before[i] + __popcll(ties & ((1ull << lane) - 1));
-        if (key[i] > bound || (key[i] == bound && nth < quota) ||
-            (reach <= KG && key[i] >= bound))
-            sh.group[atomicAdd(&sh.n_group, 1)] = i * BLOCK + tid;
+            for (int i = 0; i < NG; ++i)
+                if (key[i] >= bound) sh.group[slot++] = i * BLOCK + tid;
+        }
     }
     __syncthreads();
+    // as many as were entered (of a row with NaN it can be fewer)
+    reach = sh.n_group;
+    const int slots = reach * LPG, V = (int)g_V;
+    auto where = [&](int i) {
+        const int slot = i + tid;
+        return slot < slots ? sh.group[slot / LPG] * GROUP + slot % LPG * N : V;
+    };
+    auto vector = [&](int at) {
+        if (V < N) return load_vec(row, (long)at, (long)V);
+        Vec<T> v;
+        v.load(row + min(at, V - N));
+        const int past = min(max(at + N - V, 0), N);
+        if (__ballot(past != 0)) shift_in_pad(v, past);
+        return v;
+    };
+    // candidates into LDS, one request for slots per vector that has any;
+    // compared as floats, of which -0 equals 0
     u32 index_bound = 0xffffffffu;
-    auto collect = [&](u32 order, u32 index, bool valid) {
-        if (valid && (order > bound || (order == bound && index < index_bound))) {
-            const int slot = atomicAdd(&sh.n_key, 1);
-            if (slot < CAP) sh.key[slot] = (u64)order << 32 | ~index;
+    auto collect = [&](const Vec<T> &v, int at) {
+        const float low = Order<T>::value(bound);
+        u32 take = 0;
+#pragma unroll
+        for (int k = N - 1; k >= 0; --k)
+            take = take << 1 | (v.get(k) >= low ? 1 : 0);
+        const int valid = min(max(V - at, 0), N);
+        take &= (1u << valid) - 1;
+        if (index_bound != 0xffffffffu) {
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (v.get(k) == low && (u32)at + k >= index_bound)
+                    take &= ~(1u << k);
+        }
+        if (take) {
+            int slot = atomicAdd(&sh.n_key, __popc(take));
+            do {
+                const int k = __ffs(take) - 1;
+                take &= take - 1;
+                if (slot < CAP)
+                    sh.key[slot] = (u64)Order<T>::of(v.pick(k)) << 32 |
+                                   ~((u32)at + k);
+                ++slot;
+            } while (take);
         }
     };
-    for_candidates<T>(row, V, sh, KG, collect);
+    auto collect_all = [&](auto between) {
+#pragma unroll 1
+        for (int i0 = 0; i0 < slots; i0 += AHEAD * BLOCK) {
+            Vec<T> v[AHEAD];
+            int at[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                at[i] = where(i0 + i * BLOCK);
+                if (i0 + i * BLOCK < slots) v[i] = vector(at[i]);
+            }
+            if (i0 == 0) between();
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                if (i0 + i * BLOCK < slots) collect(v[i], at[i]);
+        }
+    };
+    collect_all(meanwhile);
     __syncthreads();
     int n = sh.n_key;
     if (n > CAP) {
-        bound = 0;
-        for (int bit = Order<T>::BITS - 1; bit >= 0; --bit) {
-            const u32 b = bound | 1u << bit;
+        auto count = [&](auto pred) {
             int c = 0;
-            for_candidates<T>(row, V, sh, KG, [&](u32 order, u32, bool valid) {
-                c += __popcll(__ballot(valid && order >= b));
-            });
-            c = block_count(c, sh, turn);
-            if (c >= K) {
-                bound = b;
-                n = c;
-                if (c <= CAP) break;
+#pragma unroll 1
+            for (int i = 0; i < slots; i += BLOCK) {
+                const int at = where(i);
+                const Vec<T> x = vector(at);
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+                    c += __popcll(
+                        __ballot(at + k < V && pred(Order<T>::of(x.get(k)),
+                                                    (u32)at + k)));
             }
-        }
+            return c;
+        };
+        bound = search_bound(Order<T>::BITS, K, CAP, n, sh, turn, [&](u32 b) {
+            return count([&](u32 order, u32) { return order >= b; });
+        });
         if (n > CAP) {
             // more than CAP tokens share the K-th value: `need` of them, the
             // first ones
-            int above = 0;
-            for_candidates<T>(row, V, sh, KG, [&](u32 order, u32, bool valid) {
-                above += __popcll(__ballot(valid && order > bound));
-            });
-            const int need = K - block_count(above, sh, turn);
+            const int above =
+                count([&](u32 order, u32) { return order > bound; });
+            const int need = K - block_count(above, 0, 0, sh, turn).x;
             index_bound = 0;
+#pragma unroll 1
             for (int bit = 30; bit >= 0; --bit) {
                 const u32 b = index_bound | 1u << bit;
-                int c = 0;
-                for_candidates<T>(
-                    row, V, sh, KG, [&](u32 order, u32 index, bool valid) {
-                        c += __popcll(__ballot(valid && order == bound &&
-                                               index < b));
-                    });
-                if (block_count(c, sh, turn) <= need) index_bound = b;
+                const int c = count([&](u32 order, u32 index) {
+                    return order == bound && index < b;
+                });
+                if (block_count(c, 0, 0, sh, turn).x <= need) index_bound = b;
             }
         }
         if (tid == 0) sh.n_key = 0;
         __syncthreads();
-        for_candidates<T>(row, V, sh, KG, collect);
+        collect_all([] {});
         __syncthreads();
         n = sh.n_key;
     }
-    for (int i = tid; i < n; i += BLOCK) {
-        const u64 mine = sh.key[i];
+    // four lanes count the better ones of each candidate, a quarter each;
+    // keys of 0 stand behind the candidates up to a multiple of 32
+    if (tid < 32 && n + tid < CAP) sh.key[n + tid] = 0;
+    __syncthreads();
+    for (int i = tid / 4; i < (n + 3) / 4 * 4; i += BLOCK / 4) {
+        const u64 mine = sh.key[min(i, CAP - 1)];
         int rank = 0;
-        for (int j = 0; j < n; ++j) rank += sh.key[j] > mine;
-        if (rank < K) {
-            const u32 index = ~(u32)mine;
-            top_ids[rank] = (long)index;
-            top_lp[rank] = none ? -INFINITY
-                                : (float)(((double)to_f(row[index]) - m) *
-                                              inv_t - ln_s);
+        for (int j = tid % 4; j < n; j += 32)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) rank += sh.key[j + 4 * k] > mine;
+        rank += dpp_i<DPP_XOR1>(rank);
+        rank += dpp_i<DPP_XOR2>(rank);
+        if (i < n && rank < K && tid % 4 == 0) {
+            top_ids[rank] = (long)(u32)~(u32)mine;
+            top_lp[rank] = Order<T>::value((u32)(mine >> 32));
         }
     }
-    __syncthreads();
 }
 
 struct RowOut {
@@ -769,35 +964,48 @@ struct RowOut {
     bool none, bad;  // no finite logit; NaN or +inf among them
 };
 
+// a row's given token, its logit, and its first stretches: asked for early
+template <typename T> struct RowIn {
+    float4 first;
+    float x;
+    bool inside;  // the token is in the vocabulary
+    DEV RowIn(const VocabRows &g, const float4 *part, int r,
+              const long *tokens, int lane) {
+        const long tok = tokens ? tokens[r] : -1;
+        inside = tok >= 0 && tok < g.V;
+        first = first_part(part + (long)r * g.nseg, g.nseg, lane);
+        x = inside ? to_f(row_ptr<T>(g, r)[tok]) : 0.f;
+    }
+};
+
 // One wave: a row's log probability, entropy and stat[r] =
 // (m, 1/s, H - ln s, 0) against the rounded m*c, what the gradient needs;
 // 1/s is 0 where the row has no finite logit.
 template <typename T>
-DEV RowOut logprobs_row(const VocabRows &g, const float4 *part, int r,
-                        const long *tokens, float c, double inv_t,
+DEV RowOut logprobs_row(const RowIn<T> &in, const VocabRows &g,
+                        const float4 *part, int r, float c, double inv_t,
                         float *logprobs, float *entropy, float4 *stat,
                         int lane, bool write) {
-    const RowStat st = join_parts(part + (long)r * g.nseg, g.nseg, c, lane);
+    const RowStat st =
+        join_parts(in.first, part + (long)r * g.nseg, g.nseg, c, lane);
     RowOut o;
     o.m = st.m;
     o.none = st.s == 0;
     o.bad = !(st.s < INFINITY);
-    o.ln_s = log(st.s);
+    o.ln_s = log_d(st.s);
     if (write && lane == 0) {
-        if (tokens) {
-            const long tok = tokens[r];
+        if (logprobs) {
             float lp = NAN;
-            if (tok >= 0 && tok < g.V && !o.bad)
+            if (in.inside && !o.bad)
                 lp = o.none ? -INFINITY
-                            : (float)(((double)to_f(row_ptr<T>(g, r)[tok]) -
-                                       o.m) * inv_t - o.ln_s);
+                            : (float)(((double)in.x - o.m) * inv_t - o.ln_s);
             logprobs[r] = lp;
         }
         const double ln2 = 0.6931471805599453, mean = st.t / st.s;
         entropy[r] = o.none ? 0.f
                      : o.bad ? NAN : (float)(o.ln_s - ln2 * mean);
         stat[r] = make_float4(
-            st.m, o.none ? 0.f : (float)(exp2(-st.delta) / st.s),
+            st.m, o.none ? 0.f : (float)(exp2_d(-st.delta) / st.s),
             o.none ? 0.f : (float)(-ln2 * (mean + st.delta)), 0.f);
     }
     return o;
@@ -806,191 +1014,246 @@ DEV RowOut logprobs_row(const VocabRows &g, const float4 *part, int r,
 // without alternatives: one wave per row
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void logprobs_join(
-    VocabRows g, const float4 *__restrict__ part,
+    VocabRows g, u32 first, const float4 *__restrict__ part,
     const long *__restrict__ tokens, long ignore, float c, double inv_t,
     float *__restrict__ logprobs, float *__restrict__ entropy,
     float4 *__restrict__ stat) {
     const int lane = threadIdx.x % WAVE;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    for (u32 r = blockIdx.x * WAVES + wid; r < (u32)g.rows;
-         r += gridDim.x * WAVES) {
-        if (tokens && tokens[r] == ignore) {
-            if (lane == 0) {
-                logprobs[r] = 0.f;
-                entropy[r] = 0.f;
-                stat[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-            continue;
+    const u32 r = first + blockIdx.x * WAVES + wid;
+    if (r >= (u32)g.rows) return;
+    if (tokens && tokens[r] == ignore) {
+        if (lane == 0) {
+            logprobs[r] = 0.f;
+            entropy[r] = 0.f;
+            stat[r] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        logprobs_row<T>(g, part, (int)r, tokens, c, inv_t, logprobs, entropy,
-                        stat, lane, true);
+        return;
     }
+    const RowIn<T> in(g, part, (int)r, tokens, lane);
+    logprobs_row(in, g, part, (int)r, c, inv_t,
+                 tokens ? logprobs : nullptr, entropy, stat, lane, true);
 }
 
 // with alternatives: one workgroup per row
 template <typename T, int NG>
-__global__ __launch_bounds__(BLOCK) void logprobs_top_join(
-    VocabRows g, const float4 *__restrict__ part,
+__global__ __launch_bounds__(BLOCK)
+
+void logprobs_top_join(
+    VocabRows g, u32 first, const float4 *__restrict__ part,
     const float *__restrict__ gmax, const long *__restrict__ tokens,
     long ignore, int K, float c, double inv_t, float *__restrict__ logprobs,
     float *__restrict__ entropy, float *__restrict__ top_lp,
     long *__restrict__ top_ids, float4 *__restrict__ stat) {
     constexpr int GPS = WAVE * NVEC * Vec<T>::N / GROUP;  // per stretch
     __shared__ TopShared sh;
+    __shared__ float lp[VOCAB_MAX_K];
+    __shared__ long id[VOCAB_MAX_K];
     const int lane = threadIdx.x % WAVE;
-    for (int r = blockIdx.x; r < g.rows; r += gridDim.x) {
-        float *lp_out = top_lp + (long)r * K;
-        long *id_out = top_ids + (long)r * K;
-        if (tokens && tokens[r] == ignore) {
-            if (threadIdx.x == 0) {
-                logprobs[r] = 0.f;
-                entropy[r] = 0.f;
-                stat[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-            for (int k = threadIdx.x; k < K; k += BLOCK) {
-                lp_out[k] = 0.f;
-                id_out[k] = -1;
-            }
-            continue;
-        }
-        // every wave joins for itself
-        const RowOut o = logprobs_row<T>(g, part, r, tokens, c, inv_t,
-                                         logprobs, entropy, stat, lane,
-                                         threadIdx.x < WAVE);
-        if (o.bad) {
-            for (int k = threadIdx.x; k < K; k += BLOCK) {
-                lp_out[k] = NAN;
-                id_out[k] = -1;
-            }
-        } else {
-            top_alternatives<T, NG>(row_ptr<T>(g, r), g.V,
-                                    gmax + (long)r * g.nseg * GPS, K, sh,
-                                    lp_out, id_out, o.m, inv_t, o.ln_s,
-                                    o.none);
-        }
+    const int r = (int)(first + blockIdx.x);
+    float *lp_out = top_lp + (long)r * K;
+    long *id_out = top_ids + (long)r * K;
+    // asked for before the token is known: a row left out has none, but
+    // the space is there
+    float gm[NG];
+    const int G = (int)((g.V + GROUP - 1) / GROUP);
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        const int k = i * BLOCK + threadIdx.x;
+        gm[i] = gmax[(long)r * g.nseg * GPS + min(k, G - 1)];
     }
+    if (tokens && tokens[r] == ignore) {
+        if (threadIdx.x == 0) {
+            logprobs[r] = 0.f;
+            entropy[r] = 0.f;
+            stat[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        for (int k = threadIdx.x; k < K; k += BLOCK) {
+            lp_out[k] = 0.f;
+            id_out[k] = -1;
+        }
+        return;
+    }
+    u32 key[NG];
+#pragma unroll
+    for (int i = 0; i < NG; ++i)
+        key[i] = i * BLOCK + (int)threadIdx.x < G ? Order<T>::of(gm[i]) : 0;
+    const RowIn<T> in(g, part, r, tokens, lane);
+    RowOut o;
+    top_alternatives<T, NG>(
+        row_ptr<T>(g, r), g.V, key, K, sh,
+        [&]() {
+            // every wave joins for itself
+            o = logprobs_row(in, g, part, r, c, inv_t,
+                             tokens ? logprobs : nullptr, entropy, stat,
+                             lane, threadIdx.x < WAVE);
+        },
+        lp, id);
+    __syncthreads();
+    for (int k = threadIdx.x; k < K; k += BLOCK) {
+        lp_out[k] = o.bad    ? NAN
+                    : o.none ? -INFINITY
+                             : (float)(((double)lp[k] - o.m) * inv_t -
+                                       o.ln_s);
+        id_out[k] = o.bad ? -1 : id[k];
+    }
+    __syncthreads();
 }
 
 // One wave per row, up to VOCAB_MAX_K / 64 entries per lane.
 // stat[r] = (m, 1/s, a_in, a_out): the gradient of a student's logit is
 // p_j a_in - sum of its q  inside the teacher's entries, p_j a_out outside.
-// Both 0 mark a row without entries. q [rows, K] is kept for the gradient.
+// Both 0 mark a row without entries. entry[r, k] = (id, q) is kept for the
+// gradient, each token once: -1 where absent or not the token's first.
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void distill_join(
-    VocabRows g, const float4 *__restrict__ part,
+    VocabRows g, u32 first, const float4 *__restrict__ part,
     const float *__restrict__ tlp, const long *__restrict__ ids, int K,
     int bucket, float c, double inv_t, float *__restrict__ loss,
-    float *__restrict__ q_out, float4 *__restrict__ stat) {
+    int2 *__restrict__ entry, float4 *__restrict__ stat) {
     constexpr int EPL = VOCAB_MAX_K / WAVE;
     constexpr int HASH = 2 * VOCAB_MAX_K;  // never more than half full
     __shared__ int seen[WAVES][HASH];
     const int lane = threadIdx.x % WAVE;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    for (u32 r = blockIdx.x * WAVES + wid; r < (u32)g.rows;
-         r += gridDim.x * WAVES) {
-        const T *row = row_ptr<T>(g, (int)r);
-        long id[EPL];
-        float l[EPL], x[EPL];
-        double q[EPL], total = 0.;
-        bool any = false, wrong = false;
+    const u32 r = first + blockIdx.x * WAVES + wid;
+    if (r >= (u32)g.rows) return;
+    const T *row = row_ptr<T>(g, (int)r);
+    const float4 *parts = part + (long)r * g.nseg;
+    const float4 first_of = first_part(parts, g.nseg, lane);
+    int id[EPL];  // -1 where absent or outside
+    float l[EPL], x[EPL];
+    double q[EPL], total = 0.;
+    bool any = false, wrong = false;
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-            const int k = e * WAVE + lane;
-            id[e] = -1;
-            l[e] = x[e] = 0.f;
-            if (k < K) {
-                id[e] = ids[(long)r * K + k];
-                l[e] = tlp[(long)r * K + k];
-            }
-        }
+    for (int e = 0; e < EPL; ++e) {
+        const int k = e * WAVE + lane;
+        const long i = k < K ? ids[(long)r * K + k] : -1;
+        l[e] = k < K ? tlp[(long)r * K + k] : 0.f;
+        any |= i >= 0;
+        wrong |= i >= g.V;
+        id[e] = i < g.V ? (int)i : -1;
+        if (i < 0) l[e] = -INFINITY;
+    }
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-            const bool held = id[e] >= 0, in = id[e] < g.V;
-            if (held && in) x[e] = to_f(row[id[e]]);
-            any |= held;
-            wrong |= held && !in;
-            q[e] = 0.;
-            if (__ballot(held)) q[e] = held ? exp((double)l[e]) : 0.;
-            total += q[e];
-        }
-        any = __ballot(any) != 0;
-        wrong = __ballot(wrong) != 0;
-        total = sum_wave_d(total);
-        double q_rest = 0., log_norm = 0., scale = 1., mass;
-        if (bucket) {
-            q_rest = total < 1. ? 1. - total : 0.;
-            mass = total + q_rest;
-        } else {
-            // not `total > 0`: NaN has to stay NaN
-            log_norm = total == 0. ? 0. : log(total);
-            scale = total == 0. ? 0. : 1. / total;
-            mass = total == 0. ? 0. : total / total;
-        }
+    for (int e = 0; e < EPL; ++e) x[e] = id[e] >= 0 ? to_f(row[id[e]]) : 0.f;
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-            q[e] *= scale;
-            const int k = e * WAVE + lane;
-            if (k < K) q_out[(long)r * K + k] = (float)q[e];
-        }
-        if (!any || (!bucket && total == 0.)) {
-            if (lane == 0) {
-                loss[r] = 0.f;
-                stat[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-            continue;
-        }
-        const RowStat st = join_parts(part + (long)r * g.nseg, g.nseg, c, lane);
-        double s = st.s;
-        if (bucket) {
-            // the listed tokens' part, each token once
-            for (int i = lane; i < HASH; i += WAVE) seen[wid][i] = -1;
-            wave_sync();
-            double s_in = 0.;
-#pragma unroll
-            for (int e = 0; e < EPL; ++e)
-                if (id[e] >= 0 && id[e] < g.V) {
-                    u32 at = ((u32)id[e] * 2654435761u) / (~0u / HASH + 1);
-                    int old;
-                    while ((old = atomicCAS(&seen[wid][at], -1, (int)id[e])) !=
-                               -1 && old != (int)id[e])
-                        at = (at + 1) % HASH;
-                    if (old == -1) s_in += exp2(((double)x[e] - st.m) * c);
-                }
-            s += sum_wave_d(s_in);
-        }
-        const bool none = s == 0, bad = !(s < INFINITY);
-        const double ln_s = log(s);
-        double sum = 0.;
+    for (int e = 0; e < EPL; ++e) {
+        q[e] = e * WAVE < K ? exp2_d(l[e] * 1.4426950408889634) : 0.;
+        total += q[e];
+    }
+    any = __ballot(any) != 0;
+    wrong = __ballot(wrong) != 0;
+    total = sum_wave_d(total);
+    double q_rest = 0., log_norm = 0., scale = 1., mass;
+    if (bucket) {
+        q_rest = total < 1. ? 1. - total : 0.;
+        mass = total + q_rest;
+    } else {
+        // not `total > 0`: NaN has to stay NaN
+        log_norm = total == 0. ? 0. : log_d(total);
+        scale = total == 0. ? 0. : 1. / total;
+        mass = total == 0. ? 0. : total / total;
+    }
+    if (!any || (!bucket && total == 0.)) {
 #pragma unroll
         for (int e = 0; e < EPL; ++e)
-            if (id[e] >= 0 && id[e] < g.V && q[e] != 0.) {
-                const double lp = none || x[e] == -INFINITY
-                                      ? -INFINITY
-                                      : ((double)x[e] - st.m) * inv_t - ln_s;
-                sum += q[e] * (((double)l[e] - log_norm) - lp);
-            }
-        sum = sum_wave_d(sum);
-        double ratio = 0.;
-        if (bucket && q_rest > 0.) {
-            // entries that cover every token with mass leave no room for
-            // the rest; what 32-bit log probabilities leave over by
-            // rounding then counts as none
-            const double p_rest = none ? 0. : st.s / s;
-            if (p_rest > 0.) {
-                ratio = q_rest / p_rest;
-                sum += q_rest * log(ratio);
-            } else if (q_rest > 0x1p-20) {
-                sum = INFINITY;
-            }
-        }
+            if (e * WAVE + lane < K)
+                entry[(long)r * K + e * WAVE + lane] = make_int2(-1, 0);
         if (lane == 0) {
-            const bool nan = bad || wrong;
-            loss[r] = nan ? NAN : (float)sum;
-            stat[r] = make_float4(st.m,
-                                  none ? 0.f : (float)(exp2(-st.delta) / s),
-                                  nan ? NAN : (float)mass,
-                                  nan ? NAN : (float)(mass - ratio));
+            loss[r] = 0.f;
+            stat[r] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
+        return;
+    }
+
+    // which entries are a token's first? By a table of the tokens seen.
+    for (int i = lane; i < HASH; i += WAVE) seen[wid][i] = -1;
+    wave_sync();
+    bool own[EPL], twice = false;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+        own[e] = id[e] >= 0;
+        if (own[e]) {
+            u32 at = ((u32)id[e] * 2654435761u) / (~0u / HASH + 1);
+            int old;
+            while ((old = atomicCAS(&seen[wid][at], -1, id[e])) != -1 &&
+                   old != id[e])
+                at = (at + 1) % HASH;
+            twice |= old != -1;
+        }
+    }
+    double weight[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) weight[e] = q[e] *= scale;
+    if (__ballot(twice)) {
+        // rare: the first in order has the sum of all, in order
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            double sum = 0.;
+            bool before = false;
+#pragma unroll
+            for (int o = 0; o < EPL; ++o) {
+#pragma unroll 1
+                for (int i = 0; i < WAVE; ++i)
+                    if (lane_i(id[o], i) == id[e]) {
+                        sum += lane_d(q[o], i);
+                        before |= o * WAVE + i < e * WAVE + lane;
+                    }
+            }
+            weight[e] = sum;
+            own[e] &= !before;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < EPL; ++e)
+        if (e * WAVE + lane < K)
+            entry[(long)r * K + e * WAVE + lane] =
+                make_int2(own[e] ? id[e] : -1,
+                          __float_as_int(own[e] ? (float)weight[e] : 0.f));
+
+    const RowStat st = join_parts(first_of, parts, g.nseg, c, lane);
+    double s = st.s;
+    if (bucket) {
+        // the listed tokens' part, each token once
+        double s_in = 0.;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e)
+            if (own[e]) s_in += exp2_d(((double)x[e] - st.m) * c);
+        s += sum_wave_d(s_in);
+    }
+    const bool none = s == 0, bad = !(s < INFINITY);
+    const double ln_s = log_d(s);
+    double sum = 0.;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e)
+        if (id[e] >= 0 && q[e] != 0.) {
+            const double lp = none || x[e] == -INFINITY
+                                  ? -INFINITY
+                                  : ((double)x[e] - st.m) * inv_t - ln_s;
+            sum += q[e] * (((double)l[e] - log_norm) - lp);
+        }
+    sum = sum_wave_d(sum);
+    double ratio = 0.;
+    if (bucket && q_rest > 0.) {
+        // entries that cover every token with mass leave no room for
+        // the rest; what 32-bit log probabilities leave over by
+        // rounding then counts as none
+        const double p_rest = none ? 0. : st.s / s;
+        if (p_rest > 0.) {
+            ratio = q_rest / p_rest;
+            sum += q_rest * log(ratio);
+        } else if (q_rest > 0x1p-20) {
+            sum = INFINITY;
+        }
+    }
+    if (lane == 0) {
+        const bool nan = bad || wrong;
+        loss[r] = nan ? NAN : (float)sum;
+        stat[r] = make_float4(st.m,
+                              none ? 0.f : (float)(exp2_d(-st.delta) / s),
+                              nan ? NAN : (float)mass,
+                              nan ? NAN : (float)(mass - ratio));
     }
 }
 
@@ -1000,188 +1263,209 @@ __global__ __launch_bounds__(BLOCK) void distill_join(
 // one or three more operations per element beside 4 or 8 bytes.
 //
 // Single tokens (the given one, alternatives with a gradient, a teacher's
-// entries) are not looked for in the pass: the entries that fall into the
-// stretch are gathered into LDS in the row's order, and after the stretch is
-// written, and its stores have arrived, each one's lane computes its token
-// anew and writes it once more. The same token given twice is added up by its
-// first entry's lane, in order.
+// entries): those of the stretch are marked in LDS, a bit and a value each,
+// while the stretch's loads are under way, and only vectors that hold one
+// look there. Entries name a token once, the forward pass has seen to that.
+//
+// What bounds it is the memory, which takes reads and writes together best
+// from few waves with little each: the values' place in LDS (33 KB) leaves
+// four workgroups to a CU, and a stretch is half as long as in the forward
+// pass. Copying alone, 8192 rows of 128257 bf16: 765 us with 8 vectors per
+// lane and eight workgroups, 703 us with 4 and four.
 template <typename T, bool DISTILL>
 __global__ __launch_bounds__(BLOCK) void vocab_grad(
-    VocabRows g, VocabGrad a, T *__restrict__ out) {
+    VocabRows g, u32 nseg, u32 first, float c, float inv_t,
+    const float4 *__restrict__ stat, const float *__restrict__ d_row,
+    const float *__restrict__ d_entropy, const long *__restrict__ tokens,
+    long ignore, const int2 *__restrict__ entry, const float *__restrict__ d_top,
+    const long *__restrict__ ids, int K, T *__restrict__ out) {
     constexpr int N = Vec<T>::N;
-    constexpr int SEG = WAVE * NVEC * N;
+    constexpr int SEG = WAVE * NGRAD * N;
+    constexpr int EPL = VOCAB_MAX_K / WAVE;
     __shared__ u32 bits_all[WAVES][SEG / 32];
-    __shared__ int at_all[WAVES][VOCAB_MAX_K + 1];
-    __shared__ float val_all[WAVES][VOCAB_MAX_K + 1];
+    __shared__ __attribute__((aligned(16))) float value_all[WAVES][SEG];
     const int lane = threadIdx.x % WAVE;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     u32 *bits = bits_all[wid];
-    int *list_at = at_all[wid];
-    float *list_val = val_all[wid];
-    const float *vals = DISTILL ? a.q : a.d_top;
-    const u32 total = (u32)g.rows * g.nseg;  // below 2^31, as is w's step
-    for (u32 w = wave_index(); w < total; w += gridDim.x * WAVES) {
-        const int r = w / (u32)g.nseg, seg = w - (u32)r * g.nseg;
-        const long lo = (long)seg * SEG;
-        const bool whole = lo + SEG <= g.V;
-        T *orow = out + (long)r * g.V;
-        const float4 st = a.stat[r];
-        bool skip = st.y == 0.f;
-        if (DISTILL) skip = skip || (st.z == 0.f && st.w == 0.f);
-        const long tok = !DISTILL && a.tokens ? a.tokens[r] : -1;
-        if (!DISTILL && a.tokens && tok == a.ignore) skip = true;
-        if (skip) {
-            const float zero[N] = {};
+    float *value = value_all[wid];
+    const u32 w = first + wave_index();  // below 2^32
+    if (w >= (u32)g.rows * nseg) return;
+    const int r = w / nseg, seg = w - r * nseg;
+    const long lo = (long)seg * SEG;
+    const bool whole = lo + SEG <= g.V;
+    T *orow = out + (long)r * g.V;
+    // the row's numbers come by scalar loads, which nothing queues behind
+    const float4 st = stat[r];
+    const long tok = !DISTILL && tokens ? tokens[r] : -1;
+    const float g_row = d_row ? d_row[r] : 0.f;
+    const float g_ent = !DISTILL && d_entropy ? d_entropy[r] : 0.f;
+    bool skip = st.y == 0.f;
+    if (DISTILL) skip = skip || (st.z == 0.f && st.w == 0.f);
+    if (!DISTILL && tokens && tok == ignore) skip = true;
+    if (skip) {
+        const float zero[N] = {};
 #pragma unroll 1
-            for (int j = 0; j < NVEC; ++j)
-                store_vec(orow, lo + (long)(j * WAVE + lane) * N, g.V, zero,
-                          whole);
-            continue;
+        for (int j = 0; j < NGRAD; ++j)
+            store_vec(orow, lo + (long)(j * WAVE + lane) * N, g.V, zero,
+                      whole);
+        return;
+    }
+    for (int i = lane; i < SEG / 32; i += WAVE) bits[i] = 0;
+    // entries before the stretch: loads arrive in order
+    const bool entries = DISTILL || d_top;
+    u32 at[EPL];  // of the stretch, SEG or more where not in it
+    float val[EPL];
+    if (entries) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            const int k = e * WAVE + lane;
+            at[e] = SEG;
+            val[e] = 0.f;
+            if (k < K) {
+                if (DISTILL) {
+                    const int2 x = entry[(long)r * K + k];
+                    at[e] = (u32)x.x - (u32)lo;
+                    val[e] = -__int_as_float(x.y);
+                } else {
+                    const u64 off = ids[(long)r * K + k] - lo;
+                    at[e] = off < SEG ? (u32)off : SEG;
+                    val[e] = d_top[(long)r * K + k];
+                }
+            }
         }
-        const T *row = row_ptr<T>(g, r);
-        Vec<T> v[NVEC];
-        load_stretch(row, lo, g.V, lane, v);
-        // e = 2^((x - m) c) counts k_out (k_in where listed) + k_d * exponent
-        int n = 0;
-        float k_in, k_out, k_d = 0.f, scale = a.inv_t;
-        if (DISTILL) {
-            scale *= a.d_row[r];
-            k_in = st.z;
-            k_out = st.w;
-        } else {
-            float gs = 0.f;
-            if (a.d_row && a.tokens) {
-                const float gr = a.d_row[r];
-                gs = tok >= 0 && tok < g.V ? gr : NAN;
-                const long at = tok - lo;
-                if (at >= 0 && at < SEG && tok < g.V) {
-                    if (lane == 0) {
-                        list_at[0] = (int)at;
-                        list_val[0] = gr;
+    }
+    const T *row = row_ptr<T>(g, r);
+    Vec<T> v[NGRAD];
+    load_stretch(row, lo, g.V, lane, v);
+
+    // e = 2^((x - m) c) counts k_out (k_in where listed) + k_d * exponent
+    float k_in = st.z, k_out = st.w, k_d = 0.f, scale = inv_t;
+    u32 tok_at = SEG;
+    if (DISTILL) {
+        scale *= g_row;
+    } else {
+        float gs = 0.f;
+        if (d_row && tokens) {
+            const bool inside = tok >= 0 && tok < g.V;
+            gs = inside ? g_row : NAN;
+            const u64 off = tok - lo;
+            if (inside && off < SEG) tok_at = (u32)off;
+        }
+        if (d_top) {
+            float gk = 0.f;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) gk += val[e];
+            gs += sum_wave(gk);
+        }
+        k_d = -g_ent;
+        k_in = k_out = k_d * st.z - gs;
+        k_d *= 0.69314718f;
+    }
+
+    // mark the listed tokens, and note which vectors hold one
+    u32 hit = 0;
+    if (entries || tok_at < SEG) {
+        wave_sync();  // the bits are clear
+        bool found = false;  // the given token among the alternatives
+        if (entries) {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e)
+                if (at[e] < SEG) {
+                    if (!DISTILL && at[e] == tok_at) {
+                        val[e] += g_row;
+                        found = true;
                     }
-                    n = 1;
+                    atomicOr(&bits[at[e] >> 5], 1u << (at[e] & 31));
+                    value[at[e]] = val[e] * scale;
+                    hit |= 1u << (at[e] / (WAVE * N));
                 }
-            }
-            if (a.d_top) {
-                float gk = 0.f;
-                for (int k = lane; k < a.K; k += WAVE)
-                    gk += a.d_top[(long)r * a.K + k];
-                gs += sum_wave(gk);
-            }
-            if (a.d_entropy) k_d = -a.d_entropy[r];
-            k_in = k_out = k_d * st.z - gs;
-            k_d *= 0.69314718f;
         }
-        if (vals) {
-            for (int k0 = 0; k0 < a.K; k0 += WAVE) {
-                const int k = k0 + lane;
-                const long at = k < a.K ? a.ids[(long)r * a.K + k] - lo : -1;
-                const bool mine = at >= 0 && at < SEG && at + lo < g.V;
-                const u64 who = __ballot(mine);
-                if (mine) {
-                    const int slot = n + __popcll(who & ((1ull << lane) - 1));
-                    const float val = vals[(long)r * a.K + k];
-                    list_at[slot] = (int)at;
-                    list_val[slot] = DISTILL ? -val : val;
-                }
-                n += __popcll(who);
-            }
+        if (!DISTILL && tok_at < SEG && __ballot(found) == 0 && lane == 0) {
+            atomicOr(&bits[tok_at >> 5], 1u << (tok_at & 31));
+            value[tok_at] = g_row * scale;
+            hit |= 1u << (tok_at / (WAVE * N));
         }
         wave_sync();
-        const float mc = st.x * a.c, u = st.y * scale;
-        const float u_out = k_out * u, u_d = k_d * u;
-        const bool product = by_product(mc);
-        auto grad = [&](float d, float uk) {
-            // 2^-300 is 0, and (-inf) * 0 would be NaN
-            if (!DISTILL) uk = fmaf(u_d, fmaxf(d, -300.f), uk);
-            return exp2_hw(d) * uk;
-        };
-        if (product) {
+        hit = or_wave(hit);
+    }
+
+    const float mc = st.x * c, u = st.y * scale;
+    const float u_in = k_in * u, u_out = k_out * u, u_d = k_d * u;
+    auto one = [&](const Vec<T> &x, int j, auto diff) {
+        float f[N];
+        const bool listed = hit >> j & 1;
+        const int p = (j * WAVE + lane) * N;
+        const u32 in = listed ? bits[p >> 5] >> (p & 31) : 0;
 #pragma unroll
-            for (int j = 0; j < NVEC; ++j) {
-                float f[N];
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    f[i] = grad(fmaf(v[j].get(i), a.c, -mc), u_out);
-                store_vec(orow, lo + (long)(j * WAVE + lane) * N, g.V, f,
-                          whole);
+        for (int i = 0; i < N; ++i) {
+            const float d = diff(x.get(i));
+            float k = u_out;
+            if (DISTILL) {
+                if (listed && in >> i & 1) k = u_in;
+            } else {
+                // 2^-300 is 0, and (-inf) * 0 would be NaN
+                k = fmaf(u_d, fmaxf(d, -300.f), k);
             }
-        } else {
+            f[i] = exp2_hw(d) * k;
+        }
+        if (listed) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                f[i] += in >> i & 1 ? value[p + i] : 0.f;
+        }
+        store_vec(orow, lo + p, g.V, f, whole);
+    };
+    if (by_product(mc)) {
+#pragma unroll
+        for (int j = 0; j < NGRAD; ++j)
+            one(v[j], j, [&](float x) { return fmaf(x, c, -mc); });
+    } else {
 #pragma unroll 1
-            for (int j = 0; j < NVEC; ++j) {
-                const long at = lo + (long)(j * WAVE + lane) * N;
-                const Vec<T> x = load_vec(row, at, g.V);
-                float f[N];
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    f[i] = grad((x.get(i) - st.x) * a.c, u_out);
-                store_vec(orow, at, g.V, f, whole);
-            }
-        }
-        if (n > 0) {
-            // is a token listed twice?
-            u64 twice = 0;
-            if (n > 1) {
-                for (int i = lane; i < SEG / 32; i += WAVE) bits[i] = 0;
-                wave_sync();
-                for (int k0 = 0; k0 < n; k0 += WAVE) {
-                    bool seen = false;
-                    if (k0 + lane < n) {
-                        const int at = list_at[k0 + lane];
-                        const u32 bit = 1u << (at & 31);
-                        seen = atomicOr(&bits[at >> 5], bit) & bit;
-                    }
-                    twice |= __ballot(seen);
-                }
-            }
-            for (int k0 = 0; k0 < n; k0 += WAVE) {
-                const int k = k0 + lane;
-                const int at = k < n ? list_at[k] : -1;
-                float val = k < n ? list_val[k] : 0.f;
-                bool first = k < n;
-                if (twice) {
-                    val = 0.f;
-                    for (int e = 0; e < n; ++e) {
-                        const bool same = list_at[e] == at;
-                        if (same) val += list_val[e];
-                        if (same && e < k) first = false;
-                    }
-                }
-                float f = 0.f;
-                if (first) {
-                    const float x = to_f(row[lo + at]);
-                    f = fmaf(val, scale,
-                             grad(product ? fmaf(x, a.c, -mc)
-                                          : (x - st.x) * a.c,
-                                  k_in * u));
-                }
-                // the stretch's own stores are to arrive first
-                if (k0 == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                if (first) orow[lo + at] = from_f<T>(f);
-            }
-        }
-        wave_sync();
+        for (int j = 0; j < NGRAD; ++j)
+            one(load_vec(row, lo + (long)(j * WAVE + lane) * N, g.V), j,
+                [&](float x) { return (x - st.x) * c; });
     }
 }
 
 // ---- launches --------------------------------------------------------------
-// grids are capped so that threads stay far below 2^32; waves then stride
-static int wave_grid(const VocabRows &g) {
-    const long blocks = CDIV((long)g.rows * g.nseg, (long)WAVES);
-    return (int)(blocks < (1l << 22) ? CDIV(blocks, 8) * 8 : (1l << 22));
+// More workgroups than MAX_GRID (threads stay far below 2^32) go in several
+// launches: a loop in the kernels would keep constants and addresses in
+// registers. Stretches' grids are a multiple of 8, see wave_index.
+#define MAX_GRID (1l << 22)
+
+template <typename F> static void launches(long blocks, int per, F f) {
+    for (long b = 0; b < blocks; b += MAX_GRID)
+        f((u32)(b * per), dim3((u32)(blocks - b < MAX_GRID ? blocks - b
+                                                           : MAX_GRID)));
 }
-static int row_grid(long blocks) {
-    return (int)(blocks < (1l << 22) ? blocks : (1l << 22));
+static long stretch_blocks(const VocabRows &g, u32 nseg) {
+    return CDIV(CDIV((long)g.rows * nseg, (long)WAVES), 8) * 8;
+}
+static long row_blocks(const VocabRows &g) {
+    return CDIV((long)g.rows, (long)WAVES);
+}
+
+template <typename T, bool ENT, bool EXCL, bool GRP>
+static void partials_t(const VocabRows &g, const long *tokens, long ignore,
+                       const long *ids, int K, float c, float *part,
+                       float *gmax, hipStream_t stream) {
+    launches(stretch_blocks(g, g.nseg), WAVES, [&](u32 first, dim3 grid) {
+        hipLaunchKernelGGL((vocab_partials<T, ENT, EXCL, GRP>), grid,
+                           dim3(BLOCK), 0, stream, g, first, tokens, ignore,
+                           ids, K, c, (float4 *)part, gmax);
+    });
 }
 
 template <typename T, int NG>
 static void logprobs_top_join_t(const VocabRows &g, const VocabLogprobs &a,
                                 float c, hipStream_t stream) {
-    hipLaunchKernelGGL((logprobs_top_join<T, NG>), dim3(row_grid(g.rows)),
-                       dim3(BLOCK), 0, stream, g, (const float4 *)a.part,
-                       a.gmax, a.tokens, a.ignore, a.K, c, 1. / a.temperature,
-                       a.logprobs, a.entropy, a.top_lp, a.top_ids,
-                       (float4 *)a.stat);
+    launches(g.rows, 1, [&](u32 first, dim3 grid) {
+        hipLaunchKernelGGL((logprobs_top_join<T, NG>), grid, dim3(BLOCK), 0,
+                           stream, g, first, (const float4 *)a.part, a.gmax,
+                           a.tokens, a.ignore, a.K, c, 1. / a.temperature,
+                           a.logprobs, a.entropy, a.top_lp, a.top_ids,
+                           (float4 *)a.stat);
+    });
 }
 
 template <typename T>
@@ -1189,21 +1473,18 @@ static void logprobs_fwd_t(const VocabRows &g, const VocabLogprobs &a,
                            hipStream_t stream) {
     const float c = (float)(1.4426950408889634 / a.temperature);
     if (a.K == 0) {
-        hipLaunchKernelGGL((vocab_partials<T, true, false, false>),
-                           dim3(wave_grid(g)), dim3(BLOCK), 0, stream, g,
-                           a.tokens, a.ignore, nullptr, 0, c,
-                           (float4 *)a.part, nullptr);
-        hipLaunchKernelGGL((logprobs_join<T>),
-                           dim3(row_grid(CDIV((long)g.rows, WAVES))),
-                           dim3(BLOCK), 0, stream, g, (const float4 *)a.part,
-                           a.tokens, a.ignore, c, 1. / a.temperature,
-                           a.logprobs, a.entropy, (float4 *)a.stat);
+        partials_t<T, true, false, false>(g, a.tokens, a.ignore, nullptr, 0, c,
+                                          a.part, nullptr, stream);
+        launches(row_blocks(g), WAVES, [&](u32 first, dim3 grid) {
+            hipLaunchKernelGGL((logprobs_join<T>), grid, dim3(BLOCK), 0,
+                               stream, g, first, (const float4 *)a.part,
+                               a.tokens, a.ignore, c, 1. / a.temperature,
+                               a.logprobs, a.entropy, (float4 *)a.stat);
+        });
         return;
     }
-    hipLaunchKernelGGL((vocab_partials<T, true, false, true>),
-                       dim3(wave_grid(g)), dim3(BLOCK), 0, stream, g,
-                       a.tokens, a.ignore, nullptr, 0, c, (float4 *)a.part,
-                       a.gmax);
+    partials_t<T, true, false, true>(g, a.tokens, a.ignore, nullptr, 0, c,
+                                     a.part, a.gmax, stream);
     // maxima per thread; more than VOCAB_MAX_TOP_V tokens are refused before
     const long per = CDIV(CDIV(g.V, (long)GROUP), (long)BLOCK);
     if (per <= 4) logprobs_top_join_t<T, 4>(g, a, c, stream);
@@ -1217,31 +1498,32 @@ static void distill_fwd_t(const VocabRows &g, const VocabDistill &a,
                           hipStream_t stream) {
     const float c = (float)(1.4426950408889634 / a.temperature);
     if (a.bucket)
-        hipLaunchKernelGGL((vocab_partials<T, false, true, false>),
-                           dim3(wave_grid(g)), dim3(BLOCK), 0, stream, g,
-                           nullptr, 0, a.ids, a.K, c, (float4 *)a.part,
-                           nullptr);
+        partials_t<T, false, true, false>(g, nullptr, 0, a.ids, a.K, c, a.part,
+                                          nullptr, stream);
     else
-        hipLaunchKernelGGL((vocab_partials<T, false, false, false>),
-                           dim3(wave_grid(g)), dim3(BLOCK), 0, stream, g,
-                           nullptr, 0, nullptr, 0, c, (float4 *)a.part,
-                           nullptr);
-    hipLaunchKernelGGL((distill_join<T>),
-                       dim3(row_grid(CDIV((long)g.rows, WAVES))), dim3(BLOCK),
-                       0, stream, g, (const float4 *)a.part, a.teacher_lp, a.ids,
-                       a.K, a.bucket, c, 1. / a.temperature, a.loss, a.q,
-                       (float4 *)a.stat);
+        partials_t<T, false, false, false>(g, nullptr, 0, nullptr, 0, c,
+                                           a.part, nullptr, stream);
+    launches(row_blocks(g), WAVES, [&](u32 first, dim3 grid) {
+        hipLaunchKernelGGL((distill_join<T>), grid, dim3(BLOCK), 0, stream, g,
+                           first, (const float4 *)a.part, a.teacher_lp, a.ids,
+                           a.K, a.bucket, c, 1. / a.temperature, a.loss,
+                           (int2 *)a.entry,
+                           (float4 *)a.stat);
+    });
 }
 
 template <typename T>
 static void grad_t(const VocabRows &g, const VocabGrad &a, int distill,
                    void *out, hipStream_t stream) {
-    if (distill)
-        hipLaunchKernelGGL((vocab_grad<T, true>), dim3(wave_grid(g)),
-                           dim3(BLOCK), 0, stream, g, a, (T *)out);
-    else
-        hipLaunchKernelGGL((vocab_grad<T, false>), dim3(wave_grid(g)),
-                           dim3(BLOCK), 0, stream, g, a, (T *)out);
+    const u32 nseg = (u32)CDIV(g.V, (long)(WAVE * NGRAD * Vec<T>::N));
+    launches(stretch_blocks(g, nseg), WAVES, [&](u32 first, dim3 grid) {
+        auto kernel = distill ? vocab_grad<T, true> : vocab_grad<T, false>;
+        hipLaunchKernelGGL(kernel, grid, dim3(BLOCK), 0, stream, g, nseg,
+                           first, a.c, a.inv_t, (const float4 *)a.stat,
+                           a.d_row, a.d_entropy, a.tokens, a.ignore,
+                           (const int2 *)a.entry, a.d_top, a.ids, a.K,
+                           (T *)out);
+    });
 }
 
 extern "C" int vocab_segment(int dtype) {

@@ -276,30 +276,30 @@ class _TopkDistillationFn(torch.autograd.Function):
         if e is None:
             loss, _ = _topk_distillation_torch(
                 logits, teacher_logprobs, teacher_ids, temperature, bucket)
-            ctx.save_for_backward(logits, teacher_ids, teacher_logprobs, None)
+            ctx.save_for_backward(logits, teacher_logprobs, teacher_ids, None)
             return loss
         stop = _record("bw_topk_distillation",
                        logits.numel() * logits.element_size())
-        loss, q, stat = e.topk_distillation_fwd(
+        loss, entry, stat = e.topk_distillation_fwd(
             logits, teacher_logprobs, teacher_ids, temperature, bucket)
         stop()
-        ctx.save_for_backward(logits, teacher_ids, q, stat)
+        ctx.save_for_backward(logits, None, entry, stat)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        logits, ids, q, stat = ctx.saved_tensors
+        logits, teacher, entry, stat = ctx.saved_tensors
         temperature, bucket = ctx.args
         if stat is None:
-            _, d = _topk_distillation_torch(logits, q, ids, temperature,
-                                            bucket)
+            _, d = _topk_distillation_torch(logits, teacher, entry,
+                                            temperature, bucket)
             d = (d * dloss.double()[..., None]).to(logits.dtype)
             return d, None, None, None, None
         stop = _record("bw_topk_distillation_bwd",
                        2 * logits.numel() * logits.element_size())
         d = _hip(logits).topk_distillation_bwd(dloss.contiguous(), logits,
-                                               ids, q, stat, temperature)
+                                               entry, stat, temperature)
         stop()
         return d, None, None, None, None
 
