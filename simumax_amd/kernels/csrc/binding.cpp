@@ -331,7 +331,12 @@ static bool vocab_rows(const torch::Tensor &x, VocabRows *g) {
     g->rows = (int)rows;
     g->inner = (int)std::max<int64_t>(dims[1].first, 1);
     const int seg = vocab_segment(vocab_dtype(x));
-    g->nseg = (int)((V + seg - 1) / seg);
+    const int64_t size = x.element_size();
+    const bool shifted = (int64_t)x.data_ptr() % 128 ||
+                         g->stride_o * size % 128 || g->stride_i * size % 128;
+    // a vocabulary at the limit leaves no room for the shift
+    g->line = shifted && V + 127 < VOCAB_MAX_TOP_V ? 127 : 0;
+    g->nseg = (int)((V + (g->line ? 127 / size : 0) + seg - 1) / seg);
     TORCH_CHECK(rows * g->nseg < (1ll << 31), rows, " rows of ", V, " logits");
     return true;
 }

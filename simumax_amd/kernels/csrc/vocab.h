@@ -16,6 +16,7 @@ struct VocabRows {
     const void *base;
     long V, stride_o, stride_i;
     int rows, inner, nseg;  // nseg: stretches per row
+    unsigned line;          // 127: stretches begin at cache lines; 0: at rows
 };
 
 struct VocabLogprobs {

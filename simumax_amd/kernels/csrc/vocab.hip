@@ -155,68 +155,91 @@ template <typename T> DEV u32 pad_word() {  // -inf, once or twice
            : std::is_same<T, bf16>::value ? 0xff80ff80u : 0xfc00fc00u;
 }
 
-// A vector of which `past` elements lie behind the row's end, taken from the
-// row's last 16 bytes: moved down, and -inf behind.
-template <typename T> DEV void shift_in_pad(Vec<T> &v, int past) {
+// A vector moved by `by` elements, down where positive, with -inf behind.
+template <typename T> DEV void move_vec(Vec<T> &v, int by) {
     const u32 pad = pad_word<T>();
-    if constexpr (sizeof(T) == 2) {
-        if (past & 1) {
+    if (by >= 0) {
+        if constexpr (sizeof(T) == 2) {
+            if (by & 1) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                v.w[k] = __builtin_amdgcn_alignbit(k < 3 ? v.w[k + 1] : pad,
-                                                   v.w[k], 16);
+                for (int k = 0; k < 4; ++k)
+                    v.w[k] = __builtin_amdgcn_alignbit(
+                        k < 3 ? v.w[k + 1] : pad, v.w[k], 16);
+            }
         }
+        const int words = by * (int)sizeof(T) / 4;
+        if (words & 1) v.w = (u32x4){v.w[1], v.w[2], v.w[3], pad};
+        if (words & 2) v.w = (u32x4){v.w[2], v.w[3], pad, pad};
+        if (words & 4) v.w = (u32x4){pad, pad, pad, pad};
+    } else {
+        if constexpr (sizeof(T) == 2) {
+            if (by & 1) {
+#pragma unroll
+                for (int k = 3; k >= 0; --k)
+                    v.w[k] = __builtin_amdgcn_alignbit(
+                        v.w[k], k > 0 ? v.w[k - 1] : pad, 16);
+            }
+        }
+        const int words = -by * (int)sizeof(T) / 4;
+        if (words & 1) v.w = (u32x4){pad, v.w[0], v.w[1], v.w[2]};
+        if (words & 2) v.w = (u32x4){pad, pad, v.w[0], v.w[1]};
+        if (words & 4) v.w = (u32x4){pad, pad, pad, pad};
     }
-    const int words = past * (int)sizeof(T) / 4;
-    if (words & 1) v.w = (u32x4){v.w[1], v.w[2], v.w[3], pad};
-    if (words & 2) v.w = (u32x4){v.w[2], v.w[3], pad, pad};
-    if (words & 4) v.w = (u32x4){pad, pad, pad, pad};
 }
 
-// `at` counts elements from the row's start; elements past its end are -inf
-template <typename T> DEV Vec<T> load_vec(const T *row, long at, long V) {
+// `at` counts elements from the row's start, and may lie before it or behind
+// its end: what is not in the row is -inf. A vector cut short is one load of
+// the nearest whole one, moved.
+template <typename T> DEV Vec<T> nearest_vec(const T *row, long at, long V) {
     constexpr int N = Vec<T>::N;
     Vec<T> v;
     if (V >= N) {
-        v.load(row + min(at, V - N));
-        shift_in_pad(v, (int)min(max(at + N - V, 0l), (long)N));
+        v.load(row + min(max(at, 0l), V - N));
     } else {
         float f[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            f[i] = at + i < V ? to_f(row[at + i]) : -INFINITY;
+        for (int i = 0; i < N; ++i) f[i] = i < V ? to_f(row[i]) : -INFINITY;
 #pragma unroll
         for (int i = 0; i < N; i += 2) v.put(i, f[i], f[i + 1]);
     }
     return v;
 }
+template <typename T> DEV int off_nearest(long at, long V) {
+    constexpr int N = Vec<T>::N;
+    const long by = at - min(max(at, 0l), max(V - N, 0l));
+    return (int)min(max(by, -(long)N), (long)N);
+}
+template <typename T> DEV Vec<T> load_vec(const T *row, long at, long V) {
+    Vec<T> v = nearest_vec(row, at, V);
+    move_vec(v, off_nearest<T>(at, V));
+    return v;
+}
 
-// a wave's stretch of a row; only a row's last one can be cut short
+// Stretches begin at a cache line (128 bytes) of what is streamed: the row's
+// first one lies up to a line before the row. Reads and, more so, writes of
+// whole lines are what the memory takes best: the gradient of 8192 rows of an
+// odd vocabulary of 128257 took 830 us, of 128384 tokens 698 us.
+DEV int before_row(const void *row, int size, u32 line) {
+    return (int)((u32)(u64)row & line) / size;
+}
+
+// a wave's stretch of a row; only a row's first and last can be cut short
 template <typename T, int NV>
 DEV void load_stretch(const T *row, long lo, long V, int lane,
                       Vec<T> (&v)[NV]) {
     constexpr int N = Vec<T>::N;
     constexpr int SEG = WAVE * NV * N;
-    if (lo + SEG <= V) {
+    if (lo >= 0 && lo + SEG <= V) {
         const T *p = row + lo + lane * N;
 #pragma unroll
         for (int j = 0; j < NV; ++j) v[j].stream_in(p + j * WAVE * N);
-    } else if (V >= N) {
-        const int rest = (int)(V - lo);  // below SEG
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int at = (j * WAVE + lane) * N;
-            v[j].load(row + lo + min(at, rest - N));
-        }
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int at = (j * WAVE + lane) * N;
-            shift_in_pad(v[j], min(max(at + N - rest, 0), N));
-        }
     } else {
-        v[0] = load_vec(row, (long)lane * N, V);
 #pragma unroll
-        for (int j = 1; j < NV; ++j) v[j].w = pad_word<T>();
+        for (int j = 0; j < NV; ++j)
+            v[j] = nearest_vec(row, lo + (j * WAVE + lane) * N, V);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            move_vec(v[j], off_nearest<T>(lo + (j * WAVE + lane) * N, V));
     }
 }
 
@@ -226,12 +249,12 @@ DEV void store_vec(T *row, long at, long V, const float *f, bool whole) {
     Vec<T> v;
 #pragma unroll
     for (int i = 0; i < N; i += 2) v.put(i, f[i], f[i + 1]);
-    if (whole || at + N <= V) {  // whole: the same for all lanes
+    if (whole || (at >= 0 && at + N <= V)) {  // whole: the same for all lanes
         v.stream_out(row + at);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (at + i < V) {
+            if (at + i >= 0 && at + i < V) {
                 if constexpr (sizeof(T) == 4)
                     row[at + i] = __uint_as_float(v.w[i]);
                 else
@@ -434,7 +457,7 @@ __global__ __launch_bounds__(BLOCK) void vocab_partials(
     const int r = w / (u32)g.nseg, seg = w - (u32)r * g.nseg;
     if (tokens && tokens[r] == ignore) return;
     const T *row = row_ptr<T>(g, r);
-    const long lo = (long)seg * SEG;
+    const long lo = (long)seg * SEG - before_row(row, sizeof(T), g.line);
     // the ids before the stretch: loads arrive in order
     constexpr int EPL = EXCL ? VOCAB_MAX_K / WAVE : 1;
     long id[EPL];
@@ -767,13 +790,13 @@ DEV bool bound_by_bins(const u32 (&key)[NG], int K, int most, u32 &bound,
 // What bounds it is latency: barriers, and the groups' loads. `meanwhile` is
 // work of the caller's that goes between those loads and their use.
 template <typename T, int NG, typename F>
-DEV void top_alternatives(const T *row, long g_V, const u32 (&key)[NG], int K,
-                          TopShared &sh, F meanwhile, float *top_lp,
+DEV void top_alternatives(const T *row, long g_V, int before, int G,
+                          const u32 (&key)[NG], int K, TopShared &sh,
+                          F meanwhile, float *top_lp,
                           long *top_ids) {
     constexpr int N = Vec<T>::N, LPG = GROUP / N;
     constexpr int AHEAD = 4;  // vectors per thread in flight
     const int tid = threadIdx.x, lane = tid % WAVE, wid = tid / WAVE;
-    const int G = (int)((g_V + GROUP - 1) / GROUP);
     int turn = 0;
     if (tid == 0) sh.n_group = sh.n_key = 0;
     u32 bound = Order<T>::of(-INFINITY);  // 0 are keys of no group
@@ -842,14 +865,17 @@ DEV void top_alternatives(const T *row, long g_V, const u32 (&key)[NG], int K,
     const int slots = reach * LPG, V = (int)g_V;
     auto where = [&](int i) {
         const int slot = i + tid;
-        return slot < slots ? sh.group[slot / LPG] * GROUP + slot % LPG * N : V;
+        return slot < slots
+                   ? sh.group[slot / LPG] * GROUP + slot % LPG * N - before
+                   : V;
     };
     auto vector = [&](int at) {
         if (V < N) return load_vec(row, (long)at, (long)V);
         Vec<T> v;
-        v.load(row + min(at, V - N));
-        const int past = min(max(at + N - V, 0), N);
-        if (__ballot(past != 0)) shift_in_pad(v, past);
+        const int near = min(max(at, 0), V - N);
+        v.load(row + near);
+        const int by = min(max(at - near, -N), N);
+        if (__ballot(by != 0)) move_vec(v, by);
         return v;
     };
     // candidates into LDS, one request for slots per vector that has any;
@@ -861,8 +887,8 @@ DEV void top_alternatives(const T *row, long g_V, const u32 (&key)[NG], int K,
 #pragma unroll
         for (int k = N - 1; k >= 0; --k)
             take = take << 1 | (v.get(k) >= low ? 1 : 0);
-        const int valid = min(max(V - at, 0), N);
-        take &= (1u << valid) - 1;
+        take &= (1u << min(max(V - at, 0), N)) - 1;
+        take &= ~0u << min(max(-at, 0), N);
         if (index_bound != 0xffffffffu) {
 #pragma unroll
             for (int k = 0; k < N; ++k)
@@ -910,8 +936,8 @@ DEV void top_alternatives(const T *row, long g_V, const u32 (&key)[NG], int K,
 #pragma unroll
                 for (int k = 0; k < N; ++k)
                     c += __popcll(
-                        __ballot(at + k < V && pred(Order<T>::of(x.get(k)),
-                                                    (u32)at + k)));
+                        __ballot(at + k >= 0 && at + k < V &&
+                                 pred(Order<T>::of(x.get(k)), (u32)at + k)));
             }
             return c;
         };
@@ -1056,7 +1082,9 @@ void logprobs_top_join(
     // asked for before the token is known: a row left out has none, but
     // the space is there
     float gm[NG];
-    const int G = (int)((g.V + GROUP - 1) / GROUP);
+    const T *row = row_ptr<T>(g, r);
+    const int before = before_row(row, sizeof(T), g.line);
+    const int G = (int)((g.V + before + GROUP - 1) / GROUP);
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
         const int k = i * BLOCK + threadIdx.x;
@@ -1081,7 +1109,7 @@ void logprobs_top_join(
     const RowIn<T> in(g, part, r, tokens, lane);
     RowOut o;
     top_alternatives<T, NG>(
-        row_ptr<T>(g, r), g.V, key, K, sh,
+        row, g.V, before, G, key, K, sh,
         [&]() {
             // every wave joins for itself
             o = logprobs_row(in, g, part, r, c, inv_t,
@@ -1291,9 +1319,9 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
     const u32 w = first + wave_index();  // below 2^32
     if (w >= (u32)g.rows * nseg) return;
     const int r = w / nseg, seg = w - r * nseg;
-    const long lo = (long)seg * SEG;
-    const bool whole = lo + SEG <= g.V;
     T *orow = out + (long)r * g.V;
+    const long lo = (long)seg * SEG - before_row(orow, sizeof(T), 127);
+    const bool whole = lo >= 0 && lo + SEG <= g.V;
     // the row's numbers come by scalar loads, which nothing queues behind
     const float4 st = stat[r];
     const long tok = !DISTILL && tokens ? tokens[r] : -1;
@@ -1445,6 +1473,11 @@ static long row_blocks(const VocabRows &g) {
     return CDIV((long)g.rows, (long)WAVES);
 }
 
+// stretches of a row; `shifted`: rows may begin within a line
+static long vocab_stretches(long V, int size, int seg, bool shifted) {
+    return CDIV(V + (shifted ? 127 / size : 0), (long)seg);
+}
+
 template <typename T, bool ENT, bool EXCL, bool GRP>
 static void partials_t(const VocabRows &g, const long *tokens, long ignore,
                        const long *ids, int K, float c, float *part,
@@ -1515,7 +1548,9 @@ static void distill_fwd_t(const VocabRows &g, const VocabDistill &a,
 template <typename T>
 static void grad_t(const VocabRows &g, const VocabGrad &a, int distill,
                    void *out, hipStream_t stream) {
-    const u32 nseg = (u32)CDIV(g.V, (long)(WAVE * NGRAD * Vec<T>::N));
+    const u32 nseg = (u32)vocab_stretches(
+        g.V, sizeof(T), WAVE * NGRAD * Vec<T>::N,
+        (long)(u64)out % 128 || g.V * sizeof(T) % 128);
     launches(stretch_blocks(g, nseg), WAVES, [&](u32 first, dim3 grid) {
         auto kernel = distill ? vocab_grad<T, true> : vocab_grad<T, false>;
         hipLaunchKernelGGL(kernel, grid, dim3(BLOCK), 0, stream, g, nseg,
