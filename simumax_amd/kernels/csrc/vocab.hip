@@ -190,11 +190,12 @@ template <typename T> DEV void move_vec(Vec<T> &v, int by) {
 // `at` counts elements from the row's start, and may lie before it or behind
 // its end: what is not in the row is -inf. A vector cut short is one load of
 // the nearest whole one, moved.
-template <typename T> DEV Vec<T> nearest_vec(const T *row, long at, long V) {
+template <typename T> DEV Vec<T> load_vec(const T *row, long at, long V) {
     constexpr int N = Vec<T>::N;
+    const long near = min(max(at, 0l), max(V - N, 0l));
     Vec<T> v;
     if (V >= N) {
-        v.load(row + min(max(at, 0l), V - N));
+        v.load(row + near);
     } else {
         float f[N];
 #pragma unroll
@@ -202,16 +203,7 @@ template <typename T> DEV Vec<T> nearest_vec(const T *row, long at, long V) {
 #pragma unroll
         for (int i = 0; i < N; i += 2) v.put(i, f[i], f[i + 1]);
     }
-    return v;
-}
-template <typename T> DEV int off_nearest(long at, long V) {
-    constexpr int N = Vec<T>::N;
-    const long by = at - min(max(at, 0l), max(V - N, 0l));
-    return (int)min(max(by, -(long)N), (long)N);
-}
-template <typename T> DEV Vec<T> load_vec(const T *row, long at, long V) {
-    Vec<T> v = nearest_vec(row, at, V);
-    move_vec(v, off_nearest<T>(at, V));
+    move_vec(v, (int)min(max(at - near, -(long)N), (long)N));
     return v;
 }
 
@@ -233,13 +225,25 @@ DEV void load_stretch(const T *row, long lo, long V, int lane,
         const T *p = row + lo + lane * N;
 #pragma unroll
         for (int j = 0; j < NV; ++j) v[j].stream_in(p + j * WAVE * N);
+    } else if (V >= N) {
+        // as load_vec, in numbers relative to the stretch
+        const int head = (int)max(-lo, 0l);
+        const int last = (int)min(V - N - lo, (long)SEG);
+        int by[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int at = (j * WAVE + lane) * N;
+            const int near = min(max(at, head), last);
+            v[j].load(row + lo + near);
+            by[j] = min(max(at - near, -N), N);
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) move_vec(v[j], by[j]);
     } else {
+        // the row is within the first vectors of its one stretch
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-            v[j] = nearest_vec(row, lo + (j * WAVE + lane) * N, V);
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-            move_vec(v[j], off_nearest<T>(lo + (j * WAVE + lane) * N, V));
+        for (int j = 0; j < NV; ++j) v[j].w = pad_word<T>();
+        v[0] = load_vec(row, lo + lane * N, V);
     }
 }
 
@@ -1341,30 +1345,40 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
     for (int i = lane; i < SEG / 32; i += WAVE) bits[i] = 0;
     // entries before the stretch: loads arrive in order
     const bool entries = DISTILL || d_top;
-    u32 at[EPL];  // of the stretch, SEG or more where not in it
+    int2 pair[EPL];
+    long id[EPL];
     float val[EPL];
-    if (entries) {
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-            const int k = e * WAVE + lane;
-            at[e] = SEG;
-            val[e] = 0.f;
-            if (k < K) {
-                if (DISTILL) {
-                    const int2 x = entry[(long)r * K + k];
-                    at[e] = (u32)x.x - (u32)lo;
-                    val[e] = -__int_as_float(x.y);
-                } else {
-                    const u64 off = ids[(long)r * K + k] - lo;
-                    at[e] = off < SEG ? (u32)off : SEG;
-                    val[e] = d_top[(long)r * K + k];
-                }
+    for (int e = 0; e < EPL; ++e) {
+        // nothing is done with them here: that would wait for each
+        const long k = (long)r * K + min(e * WAVE + lane, K - 1);
+        pair[e] = make_int2(-1, 0);
+        id[e] = -1;
+        val[e] = 0.f;
+        if (entries && e * WAVE < K) {
+            if (DISTILL) {
+                pair[e] = entry[k];
+            } else {
+                id[e] = ids[k];
+                val[e] = d_top[k];
             }
         }
     }
     const T *row = row_ptr<T>(g, r);
     Vec<T> v[NGRAD];
     load_stretch(row, lo, g.V, lane, v);
+    u32 at[EPL];  // of the stretch, SEG or more where not in it
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+        const bool on = e * WAVE + lane < K;
+        if (DISTILL) {
+            id[e] = pair[e].x;
+            val[e] = -__int_as_float(pair[e].y);
+        }
+        const u64 off = id[e] - lo;
+        at[e] = on && off < SEG && id[e] >= 0 ? (u32)off : SEG;
+        if (!on) val[e] = 0.f;
+    }
 
     // e = 2^((x - m) c) counts k_out (k_in where listed) + k_d * exponent
     float k_in = st.z, k_out = st.w, k_d = 0.f, scale = inv_t;
