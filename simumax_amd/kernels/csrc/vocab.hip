@@ -40,10 +40,7 @@ typedef unsigned long long u64;
 // ---- element types: 16 bytes at any element boundary -----------------------
 // Rows of an odd vocabulary start at any multiple of the element's size, so
 // vectors are loaded and stored with that alignment: one 16-byte access each,
-// which the hardware takes at any address. Loads and stores of whole
-// stretches are non-temporal: every byte is used once (read alone, 8192 rows
-// of 128384 bf16: 6.9 TB/s, against 6.3 with ordinary loads; copied 5.5
-// against 5.2).
+// which the hardware takes at any address.
 typedef u32 u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_mem __attribute__((aligned(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -55,6 +52,7 @@ template <typename T> struct Vec {
     u32x4 w;
 
     DEV void load(const T *p) { w = *(const u32x4_mem *)p; }
+    DEV void store(T *p) const { *(u32x4_mem *)p = w; }
     DEV void stream_in(const T *p) {
         w = __builtin_nontemporal_load((const u32x4_mem *)p);
     }
@@ -216,7 +214,7 @@ DEV int before_row(const void *row, int size, u32 line) {
 }
 
 // a wave's stretch of a row; only a row's first and last can be cut short
-template <typename T, int NV>
+template <bool STREAM, typename T, int NV>
 DEV void load_stretch(const T *row, long lo, long V, int lane,
                       Vec<T> (&v)[NV]) {
     constexpr int N = Vec<T>::N;
@@ -224,7 +222,9 @@ DEV void load_stretch(const T *row, long lo, long V, int lane,
     if (lo >= 0 && lo + SEG <= V) {
         const T *p = row + lo + lane * N;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) v[j].stream_in(p + j * WAVE * N);
+        for (int j = 0; j < NV; ++j)
+            if (STREAM) v[j].stream_in(p + j * WAVE * N);
+            else v[j].load(p + j * WAVE * N);
     } else if (V >= N) {
         // as load_vec, in numbers relative to the stretch
         const int head = (int)max(-lo, 0l);
@@ -247,14 +247,15 @@ DEV void load_stretch(const T *row, long lo, long V, int lane,
     }
 }
 
-template <typename T>
+template <bool STREAM, typename T>
 DEV void store_vec(T *row, long at, long V, const float *f, bool whole) {
     constexpr int N = Vec<T>::N;
     Vec<T> v;
 #pragma unroll
     for (int i = 0; i < N; i += 2) v.put(i, f[i], f[i + 1]);
     if (whole || (at >= 0 && at + N <= V)) {  // whole: the same for all lanes
-        v.stream_out(row + at);
+        if (STREAM) v.stream_out(row + at);
+        else v.store(row + at);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -445,7 +446,7 @@ DEV u32 wave_index() {
 //
 // What bounds it: per element one unpacking, one product, one exponential,
 // one or two sums and half an operation for the maximum, beside 2 or 4 bytes.
-template <typename T, bool ENT, bool EXCL, bool GRP>
+template <typename T, bool ENT, bool EXCL, bool GRP, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void vocab_partials(
     VocabRows g, u32 first, const long *__restrict__ tokens, long ignore,
     const long *__restrict__ ids, int K, float c, float4 *__restrict__ part,
@@ -473,7 +474,7 @@ __global__ __launch_bounds__(BLOCK) void vocab_partials(
         }
     }
     Vec<T> v[NVEC];
-    load_stretch(row, lo, g.V, lane, v);
+    load_stretch<STREAM>(row, lo, g.V, lane, v);
     // the tokens of this stretch that the teacher lists, one bit each
     u32 hit = 0;  // vectors of the stretch that hold one
     if (EXCL) {
@@ -1304,7 +1305,7 @@ __global__ __launch_bounds__(BLOCK) void distill_join(
 // four workgroups to a CU, and a stretch is half as long as in the forward
 // pass. Copying alone, 8192 rows of 128257 bf16: 765 us with 8 vectors per
 // lane and eight workgroups, 703 us with 4 and four.
-template <typename T, bool DISTILL>
+template <typename T, bool DISTILL, bool STREAM_IN, bool STREAM_OUT>
 __global__ __launch_bounds__(BLOCK) void vocab_grad(
     VocabRows g, u32 nseg, u32 first, float c, float inv_t,
     const float4 *__restrict__ stat, const float *__restrict__ d_row,
@@ -1338,8 +1339,8 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
         const float zero[N] = {};
 #pragma unroll 1
         for (int j = 0; j < NGRAD; ++j)
-            store_vec(orow, lo + (long)(j * WAVE + lane) * N, g.V, zero,
-                      whole);
+            store_vec<STREAM_OUT>(orow, lo + (long)(j * WAVE + lane) * N, g.V,
+                                  zero, whole);
         return;
     }
     for (int i = lane; i < SEG / 32; i += WAVE) bits[i] = 0;
@@ -1366,7 +1367,7 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
     }
     const T *row = row_ptr<T>(g, r);
     Vec<T> v[NGRAD];
-    load_stretch(row, lo, g.V, lane, v);
+    load_stretch<STREAM_IN>(row, lo, g.V, lane, v);
     u32 at[EPL];  // of the stretch, SEG or more where not in it
 #pragma unroll
     for (int e = 0; e < EPL; ++e) {
@@ -1455,7 +1456,7 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
             for (int i = 0; i < N; ++i)
                 f[i] += in >> i & 1 ? value[p + i] : 0.f;
         }
-        store_vec(orow, lo + p, g.V, f, whole);
+        store_vec<STREAM_OUT>(orow, lo + p, g.V, f, whole);
     };
     if (by_product(mc)) {
 #pragma unroll
@@ -1470,6 +1471,21 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
 }
 
 // ---- launches --------------------------------------------------------------
+// Whole stretches go past the caches (non-temporal) where they are too many
+// for the 256 MB that stand before the memory, and through them where what
+// ran before or comes after finds them there. Forward, backward and a sum of
+// the gradient, on logits just written, bf16, with ordinary loads and stores
+// / loads past the caches / both past them, in us:
+//    64 MB   70 /  71 /  80      128 MB  108 / 114 / 131
+//   192 MB  169 / 150 / 176      256 MB  225 / 210 / 221
+//   512 MB  445 / 417 / 410     2048 MB 1598 / 1561 / 1539
+#define STREAM_IN_ABOVE (144l << 20)
+#define STREAM_OUT_ABOVE (384l << 20)
+
+static long logits_bytes(const VocabRows &g, int size) {
+    return (long)g.rows * g.V * size;
+}
+
 // More workgroups than MAX_GRID (threads stay far below 2^32) go in several
 // launches: a loop in the kernels would keep constants and addresses in
 // registers. Stretches' grids are a multiple of 8, see wave_index.
@@ -1496,10 +1512,12 @@ template <typename T, bool ENT, bool EXCL, bool GRP>
 static void partials_t(const VocabRows &g, const long *tokens, long ignore,
                        const long *ids, int K, float c, float *part,
                        float *gmax, hipStream_t stream) {
+    auto kernel = logits_bytes(g, sizeof(T)) > STREAM_IN_ABOVE
+                      ? vocab_partials<T, ENT, EXCL, GRP, true>
+                      : vocab_partials<T, ENT, EXCL, GRP, false>;
     launches(stretch_blocks(g, g.nseg), WAVES, [&](u32 first, dim3 grid) {
-        hipLaunchKernelGGL((vocab_partials<T, ENT, EXCL, GRP>), grid,
-                           dim3(BLOCK), 0, stream, g, first, tokens, ignore,
-                           ids, K, c, (float4 *)part, gmax);
+        hipLaunchKernelGGL(kernel, grid, dim3(BLOCK), 0, stream, g, first,
+                           tokens, ignore, ids, K, c, (float4 *)part, gmax);
     });
 }
 
@@ -1565,8 +1583,16 @@ static void grad_t(const VocabRows &g, const VocabGrad &a, int distill,
     const u32 nseg = (u32)vocab_stretches(
         g.V, sizeof(T), WAVE * NGRAD * Vec<T>::N,
         (long)(u64)out % 128 || g.V * sizeof(T) % 128);
+    const long bytes = logits_bytes(g, sizeof(T));
+    auto kernel =
+        bytes > STREAM_OUT_ABOVE ? (distill ? vocab_grad<T, true, true, true>
+                                            : vocab_grad<T, false, true, true>)
+        : bytes > STREAM_IN_ABOVE
+            ? (distill ? vocab_grad<T, true, true, false>
+                       : vocab_grad<T, false, true, false>)
+            : (distill ? vocab_grad<T, true, false, false>
+                       : vocab_grad<T, false, false, false>);
     launches(stretch_blocks(g, nseg), WAVES, [&](u32 first, dim3 grid) {
-        auto kernel = distill ? vocab_grad<T, true> : vocab_grad<T, false>;
         hipLaunchKernelGGL(kernel, grid, dim3(BLOCK), 0, stream, g, nseg,
                            first, a.c, a.inv_t, (const float4 *)a.stat,
                            a.d_row, a.d_entropy, a.tokens, a.ignore,
