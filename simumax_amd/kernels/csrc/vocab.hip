@@ -731,31 +731,36 @@ DEV int scan_wave(int v) {
     return v;
 }
 
-// The same bound for the groups' maxima, from one count of how far each is
-// below the largest, in steps of a bfloat16 (eight octaves: BINS = 1024).
-// False where fewer than K are that near, or where the step's maxima are
-// more than `most` and the type has finer ones.
+// The same bound from one count of how far keys are below the largest, in
+// steps of a bfloat16 (eight octaves: BINS = 1024): clear, add, find.
 template <typename T, int NG>
-DEV bool bound_by_bins(const u32 (&key)[NG], int K, int most, u32 &bound,
-                       int &reach, TopShared &sh) {
+DEV u32 bins_clear(const u32 (&key)[NG], TopShared &sh) {
     constexpr int FINE = 16 - Order<T>::LOW;
-    const int tid = threadIdx.x, lane = tid % WAVE, wid = tid / WAVE;
+    const int tid = threadIdx.x;
     u32 top = 0;
 #pragma unroll
     for (int i = 0; i < NG; ++i) top = max(top, key[i]);
-    top >>= FINE;  // maxima are below 2^31 now: signed comparison serves
+    top >>= FINE;  // below 2^31 now: signed comparison serves
     top = (u32)max_wave((int)top);
-    if (lane == 0) sh.top[wid] = top;
+    if (tid % WAVE == 0) sh.top[tid / WAVE] = top;
     *(int4 *)&sh.bin[tid * 4] = make_int4(0, 0, 0, 0);
     if (tid == 0) sh.reach = 0;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) top = max(top, sh.top[w]);
-#pragma unroll
-    for (int i = 0; i < NG; ++i) {
-        const u32 below = top - (key[i] >> FINE);
-        if (key[i] && below < BINS) atomicAdd(&sh.bin[below], 1u);
-    }
+    return top;
+}
+template <typename T> DEV void bins_add(u32 key, u32 top, TopShared &sh) {
+    const u32 below = top - (key >> (16 - Order<T>::LOW));
+    if (key && below < BINS) atomicAdd(&sh.bin[below], 1u);
+}
+// False where fewer than K keys are that near, or where more than `most`
+// reach the K-th's step and the type has finer ones.
+template <typename T>
+DEV bool bins_find(int K, int most, u32 top, u32 &bound, int &reach,
+                   TopShared &sh) {
+    constexpr int FINE = 16 - Order<T>::LOW;
+    const int tid = threadIdx.x, lane = tid % WAVE, wid = tid / WAVE;
     __syncthreads();
     const int4 b = *(const int4 *)&sh.bin[tid * 4];
     const int own = b.x + b.y + b.z + b.w, upto = scan_wave(own);
@@ -775,9 +780,10 @@ DEV bool bound_by_bins(const u32 (&key)[NG], int K, int most, u32 &bound,
         sh.reach = n;
     }
     __syncthreads();
+    if (sh.reach == 0 || (FINE > 0 && sh.reach > most)) return false;
     bound = sh.bound;
     reach = sh.reach;
-    return reach > 0 && (FINE == 0 || reach <= most);
+    return true;
 }
 
 // The K largest of a row, (value down, index up), from its groups' maxima.
@@ -807,18 +813,19 @@ DEV void top_alternatives(const T *row, long g_V, int before, int G,
     u32 bound = Order<T>::of(-INFINITY);  // 0 are keys of no group
     int reach = G;  // how many groups reach it
     const int most = min(K + max(K / 2, 16), GROUPS);
-    if (G <= most) {
-        __syncthreads();  // n_group, n_key
-    } else if (!bound_by_bins<T, NG>(key, K, most, bound, reach, sh)) {
-        reach = G;
-        bound = search_bound(Order<T>::BITS, K, most, reach, sh, turn,
-                             [&](u32 b) {
-                                 int n = 0;
+    const u32 top = bins_clear<T, NG>(key, sh);
+    if (G > most) {
 #pragma unroll
-                                 for (int i = 0; i < NG; ++i)
-                                     n += __popcll(__ballot(key[i] >= b));
-                                 return n;
-                             });
+        for (int i = 0; i < NG; ++i) bins_add<T>(key[i], top, sh);
+        if (!bins_find<T>(K, most, top, bound, reach, sh))
+            bound = search_bound(Order<T>::BITS, K, most, reach, sh, turn,
+                                 [&](u32 b) {
+                                     int n = 0;
+#pragma unroll
+                                     for (int i = 0; i < NG; ++i)
+                                         n += __popcll(__ballot(key[i] >= b));
+                                     return n;
+                                 });
     }
     if (reach > most) {
         // `bound` is the K-th maximum: of the groups that equal it, those of
@@ -928,7 +935,13 @@ DEV void top_alternatives(const T *row, long g_V, int before, int G,
                 if (i0 + i * BLOCK < slots) collect(v[i], at[i]);
         }
     };
-    collect_all(meanwhile);
+    // a vocabulary of few groups has told nothing yet
+    if (G > most || V <= CAP) {
+        collect_all(meanwhile);
+    } else {
+        meanwhile();
+        if (tid == 0) sh.n_key = CAP + 1;
+    }
     __syncthreads();
     int n = sh.n_key;
     if (n > CAP) {
@@ -946,9 +959,21 @@ DEV void top_alternatives(const T *row, long g_V, int before, int G,
             }
             return c;
         };
-        bound = search_bound(Order<T>::BITS, K, CAP, n, sh, turn, [&](u32 b) {
-            return count([&](u32 order, u32) { return order >= b; });
-        });
+        // a count of the tokens themselves, as of the maxima before
+        bins_clear<T, NG>(key, sh);
+#pragma unroll 1
+        for (int i = 0; i < slots; i += BLOCK) {
+            const int at = where(i);
+            const Vec<T> x = vector(at);
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (at + k >= 0 && at + k < V)
+                    bins_add<T>(Order<T>::of(x.get(k)), top, sh);
+        }
+        if (!bins_find<T>(K, CAP, top, bound, n, sh))
+            bound = search_bound(Order<T>::BITS, K, CAP, n, sh, turn, [&](u32 b) {
+                return count([&](u32 order, u32) { return order >= b; });
+            });
         if (n > CAP) {
             // more than CAP tokens share the K-th value: `need` of them, the
             // first ones
