@@ -1,5 +1,6 @@
 // PyTorch bindings for the simumax_amd gfx950 kernels.
 // Compiled directly with hipcc (no hipify pass) by kernels/build.py.
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
@@ -516,6 +517,95 @@ torch::Tensor topk_distillation_bwd(torch::Tensor dloss, torch::Tensor logits,
     return out;
 }
 
+// ---- the same as differentiable operators, without Python on the way ----
+// As under once_differentiable: a gradient of the gradient raises when it is
+// asked for.
+static torch::autograd::variable_list differentiable_once(
+    torch::autograd::variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    auto tensor = grads[0];
+    tensor = tensor.detach().requires_grad_(true);
+    auto raises = std::make_shared<torch::autograd::DelayedError>(
+        "this operator is differentiable once", 1);
+    grads[0] = (*raises)({tensor})[0];
+    return grads;
+}
+
+static c10::optional<torch::Tensor> defined_or_none(const torch::Tensor &t,
+                                                    bool wanted = true) {
+    if (!wanted || !t.defined()) return c10::nullopt;
+    return t.contiguous();
+}
+
+struct TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
+    static torch::autograd::variable_list forward(
+        torch::autograd::AutogradContext *ctx, const torch::Tensor &logits,
+        const c10::optional<torch::Tensor> &tokens, int64_t topk,
+        double temperature, int64_t ignore_index) {
+        auto o = token_logprobs_fwd(logits, tokens, topk, temperature,
+                                    ignore_index);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward(
+            {logits, tokens ? *tokens : torch::Tensor(), o[3], o[4]});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["ignore_index"] = ignore_index;
+        ctx->mark_non_differentiable({o[3]});
+        return {o[0], o[1], o[2], o[3]};
+    }
+    static torch::autograd::variable_list backward(
+        torch::autograd::AutogradContext *ctx,
+        torch::autograd::variable_list d) {
+        const auto saved = ctx->get_saved_variables();
+        const auto tokens = defined_or_none(saved[1]);
+        auto grad = token_logprobs_bwd(
+            saved[0], tokens, saved[2], saved[3],
+            defined_or_none(d[0], tokens.has_value()), defined_or_none(d[1]),
+            defined_or_none(d[2], saved[2].size(-1) > 0),
+            ctx->saved_data["temperature"].toDouble(),
+            ctx->saved_data["ignore_index"].toInt());
+        return differentiable_once({grad, {}, {}, {}, {}});
+    }
+};
+
+struct TopkDistillation : public torch::autograd::Function<TopkDistillation> {
+    static torch::Tensor forward(torch::autograd::AutogradContext *ctx,
+                                 const torch::Tensor &logits,
+                                 const torch::Tensor &teacher_logprobs,
+                                 const torch::Tensor &teacher_ids,
+                                 double temperature, bool bucket) {
+        auto o = topk_distillation_fwd(logits, teacher_logprobs, teacher_ids,
+                                       temperature, bucket);
+        ctx->save_for_backward({logits, o[1], o[2]});
+        ctx->saved_data["temperature"] = temperature;
+        return o[0];
+    }
+    static torch::autograd::variable_list backward(
+        torch::autograd::AutogradContext *ctx,
+        torch::autograd::variable_list d) {
+        const auto saved = ctx->get_saved_variables();
+        auto grad = topk_distillation_bwd(
+            d[0].contiguous(), saved[0], saved[1], saved[2],
+            ctx->saved_data["temperature"].toDouble());
+        return differentiable_once({grad, {}, {}, {}, {}});
+    }
+};
+
+std::vector<torch::Tensor> token_logprobs(torch::Tensor logits,
+                                          c10::optional<torch::Tensor> tokens,
+                                          int64_t topk, double temperature,
+                                          int64_t ignore_index) {
+    return TokenLogprobs::apply(logits, tokens, topk, temperature,
+                                ignore_index);
+}
+
+torch::Tensor topk_distillation(torch::Tensor logits,
+                                torch::Tensor teacher_logprobs,
+                                torch::Tensor teacher_ids, double temperature,
+                                bool bucket) {
+    return TopkDistillation::apply(logits, teacher_logprobs, teacher_ids,
+                                   temperature, bucket);
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("fp8_cast", &fp8_cast,
           "fused bf16->fp8 cast + running amax (delayed scaling)");
@@ -539,6 +629,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "grouped expert GEMM dgrad: [E,M,N]x[E,N,K] -> [E,M,K] (MFMA)");
     m.def("grouped_wgrad", &grouped_wgrad,
           "grouped expert wgrad: fp32 G[E,N,K] += dout^T @ x (MFMA)");
+    m.def("token_logprobs", &token_logprobs,
+          "token_logprobs_fwd with its gradient (gfx950)");
+    m.def("topk_distillation", &topk_distillation,
+          "topk_distillation_fwd with its gradient (gfx950)");
     m.def("token_logprobs_fwd", &token_logprobs_fwd,
           "log probabilities, entropy, top alternatives of logits (gfx950)");
     m.def("token_logprobs_bwd", &token_logprobs_bwd,

@@ -11,6 +11,8 @@ strides: a view such as ``logits[:, :-1]`` is read in place (more than two
 strides over the rows, or a stride within a row, cost a copy). Statistics,
 losses and log probabilities are 32-bit; the gradient has the logits' type.
 No call synchronises with the host, and the same input gives the same bits.
+The autograd functions here run on the CPU and while ``insitu`` records; else
+the extension's own do the same without Python in the backward pass.
 
 What a row gives where its mask leaves little or nothing:
 
@@ -210,8 +212,11 @@ def token_logprobs(logits, tokens=None, topk=0, temperature=1.0,
     if tokens is not None:
         _check_ids("tokens", tokens, logits.shape[:-1], logits.device)
         tokens = tokens.contiguous()
-    lp, ent, top, ids = _TokenLogprobsFn.apply(
-        logits, tokens, int(topk), float(temperature), int(ignore_index))
+    args = (logits, tokens, int(topk), float(temperature), int(ignore_index))
+    if logits.is_cuda and not insitu.ENABLED:
+        lp, ent, top, ids = _hip(logits).token_logprobs(*args)
+    else:
+        lp, ent, top, ids = _TokenLogprobsFn.apply(*args)
     return TokenLogprobs(lp if tokens is not None else None, ent,
                          top if topk else None, ids if topk else None)
 
@@ -348,6 +353,8 @@ def topk_distillation(logits, teacher_logprobs, teacher_ids, temperature=1.0,
                          f"{logits.device}, not "
                          f"{tuple(teacher_logprobs.shape)} on "
                          f"{teacher_logprobs.device}")
-    return _TopkDistillationFn.apply(
-        logits, teacher_logprobs.detach().float().contiguous(),
-        teacher_ids.contiguous(), float(temperature), tail == "bucket")
+    args = (logits, teacher_logprobs.detach().float().contiguous(),
+            teacher_ids.contiguous(), float(temperature), tail == "bucket")
+    if logits.is_cuda and not insitu.ENABLED:
+        return _hip(logits).topk_distillation(*args)
+    return _TopkDistillationFn.apply(*args)
