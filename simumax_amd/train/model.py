@@ -331,8 +331,8 @@ class LlamaForTraining(nn.Module):
                                 device=device or "cpu")
         self.register_buffer("rope_cs", cs, persistent=False)
 
-    def forward(self, tokens, labels):
-        # tokens/labels: [B, S] int64 (S = the LOCAL seq slice under CP)
+    def _hidden(self, tokens):
+        # tokens: [B, S] int64 (S = the LOCAL seq slice under CP)
         B, S = tokens.shape
         if self.cp_size > 1:
             from .cp import cp_positions
@@ -360,7 +360,12 @@ class LlamaForTraining(nn.Module):
                                     use_reentrant=False)
             else:
                 x = layer(x, self.rope_cs, pos)
-        x = self.final_norm(x)
+        return self.final_norm(x)
+
+    def forward(self, tokens, labels):
+        # tokens/labels: [B, S] int64 (S = the LOCAL seq slice under CP)
+        B, S = tokens.shape
+        x = self._hidden(tokens)
         if self.tp_size > 1:
             from .tp import copy_to_tp, gather_seq, vocab_parallel_ce
 
@@ -376,6 +381,33 @@ class LlamaForTraining(nn.Module):
             loss = K.fused_cross_entropy(
                 logits.reshape(B * S, -1), labels.reshape(-1))
         return loss.mean()
+
+    def logits(self, tokens):
+        """[B, S] tokens -> [B, S, V] logits (the local sequence slice under
+        CP). A vocabulary sharded over tp has no whole rows to look at."""
+        if self.tp_size > 1:
+            raise NotImplementedError(
+                "logits of a vocabulary sharded over tp are not gathered")
+        return self.lm_head(self._hidden(tokens))
+
+    def token_logprobs(self, tokens, targets=None, topk=0, temperature=1.0,
+                       ignore_index=-100):
+        """Log probabilities of ``targets`` [B, S] after each prefix, with
+        entropies and top alternatives (kernels/vocab.py)."""
+        return K.token_logprobs(self.logits(tokens), targets, topk=topk,
+                                temperature=temperature,
+                                ignore_index=ignore_index)
+
+    def distillation_loss(self, tokens, teacher_logprobs, teacher_ids,
+                          temperature=1.0, tail="renormalize"):
+        """Mean divergence from a teacher's top log probabilities [B, S, K]
+        (as ``token_logprobs`` of the teacher gives them) over the positions
+        that have any."""
+        loss = K.topk_distillation(self.logits(tokens), teacher_logprobs,
+                                   teacher_ids, temperature=temperature,
+                                   tail=tail)
+        rows = (teacher_ids >= 0).any(-1).sum().clamp(min=1)
+        return loss.sum() / rows
 
     def num_params(self):
         return sum(p.numel() for p in self.parameters())

@@ -505,6 +505,29 @@ def train_step(model, opt, reducer, tokens, labels, micro_batch_num=1):
     return total_loss / micro_batch_num
 
 
+def distill_step(model, teacher, opt, reducer, tokens, micro_batch_num=1,
+                 topk=64, temperature=1.0, tail="renormalize"):
+    """``train_step`` from a teacher: per microbatch the teacher's pass gives
+    its topk log probabilities, and the student takes the gradient of its
+    divergence from them. Teacher and student share tokens and vocabulary;
+    neither's is sharded (tp = 1)."""
+    opt.zero_grad()
+    total_loss = 0.0
+    for mb in range(micro_batch_num):
+        reducer.reduce_this_pass = mb == micro_batch_num - 1
+        with torch.no_grad():
+            top = teacher.token_logprobs(tokens[mb], topk=topk,
+                                         temperature=temperature)
+        loss = model.distillation_loss(tokens[mb], top.top_logprobs,
+                                       top.top_ids, temperature=temperature,
+                                       tail=tail)
+        loss.backward()
+        total_loss += loss.item()
+    reducer.finalize()
+    opt.step()
+    return total_loss / micro_batch_num
+
+
 def make_synthetic_batch(vocab_size, micro_batch_num, micro_batch_size,
                          seq_len, device, seed=0):
     g = torch.Generator(device="cpu").manual_seed(seed)
