@@ -806,7 +806,8 @@ DEV void top_alternatives(const T *row, long g_V, int before, int G,
                           F meanwhile, float *top_lp,
                           long *top_ids) {
     constexpr int N = Vec<T>::N, LPG = GROUP / N;
-    constexpr int AHEAD = 4;  // vectors per thread in flight
+    // vectors per thread in flight: 128 groups of either size
+    constexpr int AHEAD = sizeof(T) == 4 ? 8 : 4;
     const int tid = threadIdx.x, lane = tid % WAVE, wid = tid / WAVE;
     int turn = 0;
     if (tid == 0) sh.n_group = sh.n_key = 0;
@@ -864,12 +865,14 @@ DEV void top_alternatives(const T *row, long g_V, int before, int G,
         int own = 0;
 #pragma unroll
         for (int i = 0; i < NG; ++i) own += key[i] >= bound;
-        if (own) {
-            int slot = atomicAdd(&sh.n_group, own);
+        // one request for slots per wave
+        const int upto = scan_wave(own);
+        int slot = 0;
+        if (lane == WAVE - 1) slot = atomicAdd(&sh.n_group, upto);
+        slot = lane_i(slot, WAVE - 1) + upto - own;
 #pragma unroll
-            for (int i = 0; i < NG; ++i)
-                if (key[i] >= bound) sh.group[slot++] = i * BLOCK + tid;
-        }
+        for (int i = 0; i < NG; ++i)
+            if (key[i] >= bound) sh.group[slot++] = i * BLOCK + tid;
     }
     __syncthreads();
     // as many as were entered (of a row with NaN it can be fewer)
@@ -881,15 +884,19 @@ DEV void top_alternatives(const T *row, long g_V, int before, int G,
                    ? sh.group[slot / LPG] * GROUP + slot % LPG * N - before
                    : V;
     };
-    auto vector = [&](int at) {
-        if (V < N) return load_vec(row, (long)at, (long)V);
+    // load_vec in two halves, so that loads can be under way together (of
+    // at least one vector of tokens)
+    auto nearest = [&](int at) {
         Vec<T> v;
-        const int near = min(max(at, 0), V - N);
-        v.load(row + near);
-        const int by = min(max(at - near, -N), N);
+        v.load(row + min(max(at, 0), V - N));
+        return v;
+    };
+    auto moved = [&](Vec<T> v, int at) {
+        const int by = min(max(at - min(max(at, 0), V - N), -N), N);
         if (__ballot(by != 0)) move_vec(v, by);
         return v;
     };
+    auto vector = [&](int at) { return moved(nearest(at), at); };
     // candidates into LDS, one request for slots per vector that has any;
     // compared as floats, of which -0 equals 0
     u32 index_bound = 0xffffffffu;
@@ -927,18 +934,23 @@ DEV void top_alternatives(const T *row, long g_V, int before, int G,
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
                 at[i] = where(i0 + i * BLOCK);
-                if (i0 + i * BLOCK < slots) v[i] = vector(at[i]);
+                if (i0 + i * BLOCK < slots) v[i] = nearest(at[i]);
             }
             if (i0 == 0) between();
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i)
-                if (i0 + i * BLOCK < slots) collect(v[i], at[i]);
+                if (i0 + i * BLOCK < slots) collect(moved(v[i], at[i]), at[i]);
         }
     };
-    // a vocabulary of few groups has told nothing yet
-    if (G > most || V <= CAP) {
+    if (V < N) {
+        meanwhile();
+        if (tid < V)
+            sh.key[tid] = (u64)Order<T>::of(to_f(row[tid])) << 32 | ~(u32)tid;
+        if (tid == 0) sh.n_key = V;
+    } else if (G > most || V <= CAP) {
         collect_all(meanwhile);
     } else {
+        // a vocabulary of few groups: their maxima have told nothing
         meanwhile();
         if (tid == 0) sh.n_key = CAP + 1;
     }
