@@ -798,16 +798,14 @@ DEV bool bins_find(int K, int most, u32 top, u32 &bound, int &reach,
 // searched among the tokens themselves, and, where one value alone has too
 // many, a bound on the index. The whole takes NG maxima per thread.
 //
-// What bounds it is latency: barriers, and the groups' loads. `meanwhile` is
-// work of the caller's that goes between those loads and their use.
-template <typename T, int NG, typename F>
+// What bounds it is latency: barriers, and the groups' loads.
+template <typename T, int NG>
 DEV void top_alternatives(const T *row, long g_V, int before, int G,
                           const u32 (&key)[NG], int K, TopShared &sh,
-                          F meanwhile, float *top_lp,
-                          long *top_ids) {
+                          float *top_lp, long *top_ids) {
     constexpr int N = Vec<T>::N, LPG = GROUP / N;
-    // vectors per thread in flight: 128 groups of either size
-    constexpr int AHEAD = sizeof(T) == 4 ? 8 : 4;
+    // vectors per thread in flight
+    constexpr int AHEAD = 4;
     const int tid = threadIdx.x, lane = tid % WAVE, wid = tid / WAVE;
     int turn = 0;
     if (tid == 0) sh.n_group = sh.n_key = 0;
@@ -926,7 +924,7 @@ DEV void top_alternatives(const T *row, long g_V, int before, int G,
             } while (take);
         }
     };
-    auto collect_all = [&](auto between) {
+    auto collect_all = [&]() {
 #pragma unroll 1
         for (int i0 = 0; i0 < slots; i0 += AHEAD * BLOCK) {
             Vec<T> v[AHEAD];
@@ -936,22 +934,19 @@ DEV void top_alternatives(const T *row, long g_V, int before, int G,
                 at[i] = where(i0 + i * BLOCK);
                 if (i0 + i * BLOCK < slots) v[i] = nearest(at[i]);
             }
-            if (i0 == 0) between();
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i)
                 if (i0 + i * BLOCK < slots) collect(moved(v[i], at[i]), at[i]);
         }
     };
     if (V < N) {
-        meanwhile();
         if (tid < V)
             sh.key[tid] = (u64)Order<T>::of(to_f(row[tid])) << 32 | ~(u32)tid;
         if (tid == 0) sh.n_key = V;
     } else if (G > most || V <= CAP) {
-        collect_all(meanwhile);
+        collect_all();
     } else {
         // a vocabulary of few groups: their maxima have told nothing
-        meanwhile();
         if (tid == 0) sh.n_key = CAP + 1;
     }
     __syncthreads();
@@ -1004,7 +999,7 @@ DEV void top_alternatives(const T *row, long g_V, int before, int G,
         }
         if (tid == 0) sh.n_key = 0;
         __syncthreads();
-        collect_all([] {});
+        collect_all();
         __syncthreads();
         n = sh.n_key;
     }
@@ -1053,7 +1048,7 @@ template <typename T>
 DEV RowOut logprobs_row(const RowIn<T> &in, const VocabRows &g,
                         const float4 *part, int r, float c, double inv_t,
                         float *logprobs, float *entropy, float4 *stat,
-                        int lane, bool write) {
+                        int lane) {
     const RowStat st =
         join_parts(in.first, part + (long)r * g.nseg, g.nseg, c, lane);
     RowOut o;
@@ -1061,7 +1056,7 @@ DEV RowOut logprobs_row(const RowIn<T> &in, const VocabRows &g,
     o.none = st.s == 0;
     o.bad = !(st.s < INFINITY);
     o.ln_s = log_d(st.s);
-    if (write && lane == 0) {
+    if (lane == 0) {
         if (logprobs) {
             float lp = NAN;
             if (in.inside && !o.bad)
@@ -1100,7 +1095,7 @@ __global__ __launch_bounds__(BLOCK) void logprobs_join(
     }
     const RowIn<T> in(g, part, (int)r, tokens, lane);
     logprobs_row(in, g, part, (int)r, c, inv_t,
-                 tokens ? logprobs : nullptr, entropy, stat, lane, true);
+                 tokens ? logprobs : nullptr, entropy, stat, lane);
 }
 
 // with alternatives: one workgroup per row
@@ -1115,6 +1110,7 @@ void logprobs_top_join(
     long *__restrict__ top_ids, float4 *__restrict__ stat) {
     constexpr int GPS = WAVE * NVEC * Vec<T>::N / GROUP;  // per stretch
     __shared__ TopShared sh;
+    __shared__ RowOut joined;
     __shared__ float lp[VOCAB_MAX_K];
     __shared__ long id[VOCAB_MAX_K];
     const int lane = threadIdx.x % WAVE;
@@ -1149,25 +1145,22 @@ void logprobs_top_join(
     for (int i = 0; i < NG; ++i)
         key[i] = i * BLOCK + (int)threadIdx.x < G ? Order<T>::of(gm[i]) : 0;
     const RowIn<T> in(g, part, r, tokens, lane);
-    RowOut o;
-    top_alternatives<T, NG>(
-        row, g.V, before, G, key, K, sh,
-        [&]() {
-            // every wave joins for itself
-            o = logprobs_row(in, g, part, r, c, inv_t,
-                             tokens ? logprobs : nullptr, entropy, stat,
-                             lane, threadIdx.x < WAVE);
-        },
-        lp, id);
+    top_alternatives<T, NG>(row, g.V, before, G, key, K, sh, lp, id);
+    // the first wave joins, for all: here, where nothing else is held
+    if (threadIdx.x < WAVE) {
+        const RowOut own =
+            logprobs_row(in, g, part, r, c, inv_t, tokens ? logprobs : nullptr,
+                         entropy, stat, lane);
+        if (lane == 0) joined = own;
+    }
     __syncthreads();
+    const RowOut o = joined;
     for (int k = threadIdx.x; k < K; k += BLOCK) {
         lp_out[k] = o.bad    ? NAN
                     : o.none ? -INFINITY
-                             : (float)(((double)lp[k] - o.m) * inv_t -
-                                       o.ln_s);
+                             : (float)(((double)lp[k] - o.m) * inv_t - o.ln_s);
         id_out[k] = o.bad ? -1 : id[k];
     }
-    __syncthreads();
 }
 
 // One wave per row, up to VOCAB_MAX_K / 64 entries per lane.

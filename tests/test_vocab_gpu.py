@@ -451,3 +451,141 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         e.topk_distillation_fwd(x, torch.zeros(2, 3, device=DEV).half(),
                                 ids, 1.0, True)
+
+
+def test_in_situ_timing_takes_the_same_kernels():
+    # while it records, the Python autograd functions run instead of the
+    # extension's own
+    from simumax_amd.kernels import insitu
+
+    gen = _gen(81)
+    rows, V, k = 5, 9001, 12
+    x = R.make_logits(rows, V, BF, gen)
+    tok = torch.randint(0, V, (rows,), generator=gen)
+    tlp, tid = R.make_teacher(x, k, 1.0, gen)
+    grads = (torch.randn(rows, generator=gen), torch.rand(rows, generator=gen),
+             torch.randn(rows, k, generator=gen))
+
+    def both():
+        out, d = run_logprobs(x, tok, k, 1.0, grads)
+        loss, dd = run_distill(x, tlp, tid, 1.0, "bucket", grads[0])
+        return [*out, d, loss, dd]
+
+    want = both()
+    insitu.enable()
+    try:
+        got = both()
+        recorded = {t for t, _ in insitu._RECORDS}
+    finally:
+        insitu.disable()
+        insitu._RECORDS.clear()
+    assert recorded == {"bw_token_logprobs", "bw_token_logprobs_bwd",
+                        "bw_topk_distillation", "bw_topk_distillation_bwd"}
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_a_gradient_of_the_gradient_raises():
+    x = torch.randn(2, 40, device=DEV, requires_grad=True)
+    ids = torch.zeros(2, 1, dtype=torch.int64, device=DEV)
+    for loss in (K.token_logprobs(x, ids[:, 0]).logprobs.sum(),
+                 K.topk_distillation(x, ids.float(), ids).sum()):
+        d, = torch.autograd.grad(loss, x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            d.sum().backward()
+
+
+def test_tokens_and_entries_from_an_inference_pass():
+    # a teacher under inference_mode or no_grad feeds a student that trains
+    gen = _gen(82)
+    x = R.make_logits(3, 5000, BF, gen).to(DEV)
+    with torch.inference_mode():
+        top = K.token_logprobs(x, topk=8)
+    lp, ids = top.top_logprobs.clone(), top.top_ids.clone()
+    xg = x.clone().requires_grad_(True)
+    K.topk_distillation(xg, lp, ids, tail="bucket").sum().backward()
+    # nothing to learn from itself: p - q, each off by its rounding
+    assert xg.grad.abs().max() <= 2 ** -7
+    with torch.no_grad():
+        assert not K.token_logprobs(xg, ids[:, 0]).logprobs.requires_grad
+
+
+def test_backward_into_leaves_captured():
+    """loss.backward() of a leaf, captured and replayed: the gradient that it
+    accumulates into is the graph's own memory."""
+    gen = _gen(83)
+    rows, V = 6, 7001
+    x = R.make_logits(rows, V, FP, gen).to(DEV)
+    tok = torch.randint(0, V, (rows,), generator=gen).to(DEV)
+    leaf = x.clone().requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            leaf.grad = None
+            K.token_logprobs(leaf, tok).logprobs.sum().backward()
+    torch.cuda.current_stream().wait_stream(side)
+    leaf.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        K.token_logprobs(leaf, tok).logprobs.sum().backward()
+    for turn in range(3):
+        new = R.make_logits(rows, V, FP, _gen(84 + turn)).to(DEV)
+        with torch.no_grad():
+            leaf.copy_(new)
+        graph.replay()
+        eager = new.clone().requires_grad_(True)
+        d, = torch.autograd.grad(
+            K.token_logprobs(eager, tok).logprobs.sum(), eager)
+        torch.cuda.synchronize()
+        assert torch.equal(leaf.grad, d)
+
+
+@pytest.mark.parametrize("kind", ["clustered", "equal", "masked", "steps"])
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("V,topk", [(700, 256), (5743, 256), (12345, 200),
+                                    (24571, 256)])
+def test_alternatives_of_few_groups(kind, dtype, V, topk):
+    """Vocabularies whose groups are hardly more than the alternatives."""
+    gen = _gen(91 + V)
+    x = torch.randn(3, V, generator=gen) * 2
+    if kind == "clustered":
+        x[:, V // 3:V // 3 + 400] += 9
+    elif kind == "equal":
+        x = torch.where(torch.rand(3, V, generator=gen) < 0.5, 3.25, 3.0)
+    elif kind == "masked":
+        x[torch.rand(3, V, generator=gen) < 0.97] = -math.inf
+    else:
+        # far more octaves than the first count looks at
+        x = torch.exp2(torch.randint(-30, 3, (3, V), generator=gen).float())
+    x = x.to(dtype)
+    out = K.token_logprobs(x.to(DEV), topk=topk)
+    R.check_logprobs(x, None, topk, 1.0, out)
+
+
+def test_rows_of_every_alignment():
+    """The same row at each of the 64 places within a cache line that a bf16
+    row can begin at, read and written."""
+    gen = _gen(95)
+    for V in (3, 130, 4093, 8200):
+        row = R.make_logits(1, V, BF, gen)
+        tok = torch.full((64,), V // 2)
+        tlp, tid = R.make_teacher(row, min(V, 9), 1.0, gen)
+        store = torch.zeros(64 * (V + 129) + 64, dtype=BF, device=DEV)
+        # rows of a stride that is 1 past a whole number of lines
+        stride = (V + 63) // 64 * 64 + 1
+        x = store.as_strided((64, V), (stride, 1))
+        x.copy_(row.to(DEV).expand(64, V))
+        k = min(V, 9)
+        xg = x.detach().requires_grad_(True)
+        out = K.token_logprobs(xg, tok.to(DEV), topk=k)
+        loss = K.topk_distillation(xg, tlp.to(DEV).expand(64, k),
+                                   tid.to(DEV).expand(64, k), tail="bucket")
+        g = torch.ones(64, device=DEV)
+        d1, = torch.autograd.grad((out.logprobs, out.entropy), xg, (g, g))
+        d2, = torch.autograd.grad(loss, xg, g)
+        one = torch.ones(64)
+        cpu = row.expand(64, V)
+        R.check_logprobs(cpu, tok, k, 1.0, out, (one, one, None), d1)
+        R.check_distill(cpu, tlp.expand(64, k), tid.expand(64, k), 1.0,
+                        "bucket", loss, d2, one)
