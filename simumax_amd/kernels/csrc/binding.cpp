@@ -392,9 +392,10 @@ std::vector<torch::Tensor> token_logprobs_fwd(
         torch::Tensor gmax;
         if (topk > 0)
             gmax = torch::empty({g.rows, g.nseg,
-                                 vocab_segment(dt) / vocab_group()}, f32);
+                                 vocab_segment(dt) / vocab_group()},
+                                logits.options());
         VocabLogprobs a;
-        a.gmax = topk > 0 ? gmax.data_ptr<float>() : nullptr;
+        a.gmax = topk > 0 ? gmax.data_ptr() : nullptr;
         a.tokens = tokens ? tokens->data_ptr<int64_t>() : nullptr;
         a.ignore = ignore_index;
         a.K = (int)topk;

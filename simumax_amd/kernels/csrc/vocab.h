@@ -25,7 +25,8 @@ struct VocabLogprobs {
     int K;
     double temperature;
     float *part;  // [rows, nseg, 4] workspace
-    float *gmax;  // [rows, nseg, segment / group] workspace, where K > 0
+    void *gmax;   // [rows, nseg, segment / group] of the logits' type:
+                  // workspace, where K > 0
     float *logprobs, *entropy, *top_lp;
     long *top_ids;
     float *stat;  // [rows, 4]

@@ -139,6 +139,8 @@ template <> struct Patterns<float> {
     DEV int top() const { return hi; }
     DEV u32 bottom() const { return lo; }
 };
+template <typename T> struct Pattern { typedef unsigned short type; };
+template <> struct Pattern<float> { typedef u32 type; };
 template <typename T> DEV float from_pattern(u32 bits);
 template <> DEV float from_pattern<float>(u32 b) { return __uint_as_float(b); }
 template <> DEV float from_pattern<bf16>(u32 b) {
@@ -450,7 +452,7 @@ template <typename T, bool ENT, bool EXCL, bool GRP, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void vocab_partials(
     VocabRows g, u32 first, const long *__restrict__ tokens, long ignore,
     const long *__restrict__ ids, int K, float c, float4 *__restrict__ part,
-    float *__restrict__ gmax) {
+    typename Pattern<T>::type *__restrict__ gmax) {
     constexpr int N = Vec<T>::N;
     constexpr int SEG = WAVE * NVEC * N;
     constexpr int LPG = GROUP / N;  // lanes per group: 8 or 16
@@ -512,7 +514,7 @@ __global__ __launch_bounds__(BLOCK) void vocab_partials(
             // lane (group q of a vector, j) has group j * (64 / LPG) + q
             const int q = lane / LPG, j = lane % LPG;
             gmax[(long)w * (SEG / GROUP) + j * (WAVE / LPG) + q] =
-                from_pattern<T>(gbits);
+                (typename Pattern<T>::type)gbits;
         }
         top = max_wave(mine ? gm : -2147483647 - 1);
         m_bits = (u32)top;
@@ -1100,11 +1102,9 @@ __global__ __launch_bounds__(BLOCK) void logprobs_join(
 
 // with alternatives: one workgroup per row
 template <typename T, int NG>
-__global__ __launch_bounds__(BLOCK)
-
-void logprobs_top_join(
+__global__ __launch_bounds__(BLOCK) void logprobs_top_join(
     VocabRows g, u32 first, const float4 *__restrict__ part,
-    const float *__restrict__ gmax, const long *__restrict__ tokens,
+    const typename Pattern<T>::type *__restrict__ gmax, const long *__restrict__ tokens,
     long ignore, int K, float c, double inv_t, float *__restrict__ logprobs,
     float *__restrict__ entropy, float *__restrict__ top_lp,
     long *__restrict__ top_ids, float4 *__restrict__ stat) {
@@ -1119,7 +1119,7 @@ void logprobs_top_join(
     long *id_out = top_ids + (long)r * K;
     // asked for before the token is known: a row left out has none, but
     // the space is there
-    float gm[NG];
+    typename Pattern<T>::type gm[NG];
     const T *row = row_ptr<T>(g, r);
     const int before = before_row(row, sizeof(T), g.line);
     const int G = (int)((g.V + before + GROUP - 1) / GROUP);
@@ -1143,7 +1143,7 @@ void logprobs_top_join(
     u32 key[NG];
 #pragma unroll
     for (int i = 0; i < NG; ++i)
-        key[i] = i * BLOCK + (int)threadIdx.x < G ? Order<T>::of(gm[i]) : 0;
+        key[i] = i * BLOCK + (int)threadIdx.x < G ? Order<T>::of(from_pattern<T>(gm[i])) : 0;
     const RowIn<T> in(g, part, r, tokens, lane);
     top_alternatives<T, NG>(row, g.V, before, G, key, K, sh, lp, id);
     // the first wave joins, for all: here, where nothing else is held
@@ -1541,13 +1541,14 @@ static long vocab_stretches(long V, int size, int seg, bool shifted) {
 template <typename T, bool ENT, bool EXCL, bool GRP>
 static void partials_t(const VocabRows &g, const long *tokens, long ignore,
                        const long *ids, int K, float c, float *part,
-                       float *gmax, hipStream_t stream) {
+                       void *gmax, hipStream_t stream) {
     auto kernel = logits_bytes(g, sizeof(T)) > STREAM_IN_ABOVE
                       ? vocab_partials<T, ENT, EXCL, GRP, true>
                       : vocab_partials<T, ENT, EXCL, GRP, false>;
     launches(stretch_blocks(g, g.nseg), WAVES, [&](u32 first, dim3 grid) {
         hipLaunchKernelGGL(kernel, grid, dim3(BLOCK), 0, stream, g, first,
-                           tokens, ignore, ids, K, c, (float4 *)part, gmax);
+                           tokens, ignore, ids, K, c, (float4 *)part,
+                           (typename Pattern<T>::type *)gmax);
     });
 }
 
@@ -1556,10 +1557,10 @@ static void logprobs_top_join_t(const VocabRows &g, const VocabLogprobs &a,
                                 float c, hipStream_t stream) {
     launches(g.rows, 1, [&](u32 first, dim3 grid) {
         hipLaunchKernelGGL((logprobs_top_join<T, NG>), grid, dim3(BLOCK), 0,
-                           stream, g, first, (const float4 *)a.part, a.gmax,
-                           a.tokens, a.ignore, a.K, c, 1. / a.temperature,
-                           a.logprobs, a.entropy, a.top_lp, a.top_ids,
-                           (float4 *)a.stat);
+                           stream, g, first, (const float4 *)a.part,
+                           (const typename Pattern<T>::type *)a.gmax, a.tokens,
+                           a.ignore, a.K, c, 1. / a.temperature, a.logprobs,
+                           a.entropy, a.top_lp, a.top_ids, (float4 *)a.stat);
     });
 }
 
