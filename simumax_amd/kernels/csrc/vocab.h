@@ -38,7 +38,7 @@ struct VocabDistill {
     int K, bucket;
     double temperature;
     float *part, *loss, *stat;
-    int *entry;  // [rows, K, 2]: id or -1, and the weight's bits
+    int *entry;  // [rows, K, 2]: id or -1, and its gradient's bits
 };
 
 struct VocabGrad {

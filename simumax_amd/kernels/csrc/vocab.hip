@@ -70,6 +70,7 @@ template <typename T> struct Vec {
         if constexpr (PER == 2) one.w[0] >>= (i & 1) * 16;
         return one.get(0);
     }
+    DEV void drop(u32 in);  // -inf where `in` has the element's bit
     // Largest and smallest bit pattern, as signed and unsigned numbers: of
     // floats of which one at least is not negative the first is the largest
     // float, of negative floats the second is. Packed, a half operation per
@@ -153,6 +154,20 @@ template <> DEV float from_pattern<__half>(u32 b) {
 template <typename T> DEV u32 pad_word() {  // -inf, once or twice
     return sizeof(T) == 4                       ? 0xff800000u
            : std::is_same<T, bf16>::value ? 0xff80ff80u : 0xfc00fc00u;
+}
+
+template <typename T> DEV void Vec<T>::drop(u32 in) {
+    constexpr int PER = N / 4;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        // all ones where dropped
+        u32 mask = (u32)((int)(in << (31 - k * PER)) >> 31);
+        if constexpr (PER == 2) {
+            const u32 odd = (u32)((int)(in << (30 - k * PER)) >> 31);
+            mask = (mask & 0xffffu) | odd << 16;
+        }
+        w[k] = (w[k] & ~mask) | (pad_word<T>() & mask);
+    }
 }
 
 // A vector moved by `by` elements, down where positive, with -inf behind.
@@ -440,11 +455,12 @@ DEV u32 wave_index() {
     return __builtin_amdgcn_readfirstlane(b * WAVES + threadIdx.x / WAVE);
 }
 
-// One wave per stretch. Writes (m, s, t, 0). With EXCL the sum leaves out the
-// tokens that a teacher lists (m does not): the rest of the mass is summed,
-// not got as a difference, because a student that has learned leaves little
-// of it. Only vectors that hold such a token look at its bits. With GRP also the maximum of each GROUP
-// consecutive tokens, for the search of the top alternatives.
+// One wave per stretch. Writes (m, s, t, 0). With EXCL as if the tokens that a
+// teacher lists were not there: the rest of the mass is summed against its
+// own maximum, not got as a difference, because a student that has learned
+// leaves little of it. Only vectors that hold such a token look at its bits.
+// With GRP also the maximum of each GROUP consecutive tokens, for the search
+// of the top alternatives.
 //
 // What bounds it: per element one unpacking, one product, one exponential,
 // one or two sums and half an operation for the maximum, beside 2 or 4 bytes.
@@ -479,6 +495,10 @@ __global__ __launch_bounds__(BLOCK) void vocab_partials(
     load_stretch<STREAM>(row, lo, g.V, lane, v);
     // the tokens of this stretch that the teacher lists, one bit each
     u32 hit = 0;  // vectors of the stretch that hold one
+    auto drop_listed = [&](Vec<T> &x, int j) {
+        const int at = (j * WAVE + lane) * N;
+        if (EXCL && hit >> j & 1) x.drop(bits[wid][at >> 5] >> (at & 31));
+    };
     if (EXCL) {
         for (int i = lane; i < SEG / 32; i += WAVE) bits[wid][i] = 0;
         wave_sync();
@@ -492,6 +512,8 @@ __global__ __launch_bounds__(BLOCK) void vocab_partials(
         }
         wave_sync();
         hit = or_wave(hit);
+#pragma unroll
+        for (int j = 0; j < NVEC; ++j) drop_listed(v[j], j);
     }
     // the largest value, by bit patterns; a stretch (or a group) without
     // a value >= 0 is looked at a second time
@@ -536,38 +558,27 @@ __global__ __launch_bounds__(BLOCK) void vocab_partials(
     const float mr = m == -INFINITY ? 0.f : m, mc = mr * c;
     float s = 0.f, t = 0.f;
     // one vector; the values stay packed until here
-    auto sums = [&](const Vec<T> &x, int j, auto diff) {
-        if (!EXCL || !(hit >> j & 1)) {
+    auto sums = [&](const Vec<T> &x, auto diff) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float d = diff(x.get(i)), e = exp2_hw(d);
-                s += e;
-                // 2^-300 is 0, and (-inf) * 0 would be NaN; NaN is in e
-                // already
-                if (ENT) t = fmaf(fmaxf(d, -300.f), e, t);
-            }
-        } else {
-            const int at = (j * WAVE + lane) * N;
-            const u32 in = bits[wid][at >> 5] >> (at & 31);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const u32 e = __float_as_uint(exp2_hw(diff(x.get(i))));
-                // all ones where listed
-                const u32 mask = (u32)((int)(in << (31 - i)) >> 31);
-                s += __uint_as_float(e & ~mask);
-            }
+        for (int i = 0; i < N; ++i) {
+            const float d = diff(x.get(i)), e = exp2_hw(d);
+            s += e;
+            // 2^-300 is 0, and (-inf) * 0 would be NaN; NaN is in e already
+            if (ENT) t = fmaf(fmaxf(d, -300.f), e, t);
         }
     };
     if (by_product(mc)) {
 #pragma unroll
         for (int j = 0; j < NVEC; ++j)
-            sums(v[j], j, [&](float x) { return fmaf(x, c, -mc); });
+            sums(v[j], [&](float x) { return fmaf(x, c, -mc); });
     } else {
         // rare: read again, one vector at a time, rather than held twice
 #pragma unroll 1
-        for (int j = 0; j < NVEC; ++j)
-            sums(load_vec(row, lo + (long)(j * WAVE + lane) * N, g.V), j,
-                 [&](float x) { return (x - mr) * c; });
+        for (int j = 0; j < NVEC; ++j) {
+            Vec<T> x = load_vec(row, lo + (long)(j * WAVE + lane) * N, g.V);
+            drop_listed(x, j);
+            sums(x, [&](float x) { return (x - mr) * c; });
+        }
     }
     s = sum_wave(s);
     if (ENT) t = sum_wave(t);
@@ -604,6 +615,9 @@ DEV double log_d(double v) {
     const double r = fma(v, exp2_d(-y), -1.);
     return fma(y, 0.6931471805599453, r - r * r * (0.5 - r * (1. / 3.)));
 }
+
+// sums of probabilities up to this one count as none
+#define VOCAB_NO_MASS 1e-300
 
 struct RowStat {
     float m;           // largest logit, 0 where there is none
@@ -1163,11 +1177,14 @@ __global__ __launch_bounds__(BLOCK) void logprobs_top_join(
     }
 }
 
-// One wave per row, up to VOCAB_MAX_K / 64 entries per lane.
-// stat[r] = (m, 1/s, a_in, a_out): the gradient of a student's logit is
-// p_j a_in - sum of its q  inside the teacher's entries, p_j a_out outside.
-// Both 0 mark a row without entries. entry[r, k] = (id, q) is kept for the
-// gradient, each token once: -1 where absent or not the token's first.
+// One wave per row, up to VOCAB_MAX_K / 64 entries per lane. The gradient of a
+// student's logit for a loss that counts 1 (and T = 1) is
+//   p_j mass - q_j              of a token that the teacher lists,
+//   p_j (mass - q_rest/p_rest)  of another, with q_rest = 0 without bucket.
+// entry[r, k] = (id, the former), each token once: -1 where absent or not the
+// token's first. stat[r] = (m, a, live, 0), where the latter is a 2^(x*c - mc)
+// against the largest of the others: p_rest can be far below what 32 bits
+// hold. live is 0 where the row has no gradient.
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void distill_join(
     VocabRows g, u32 first, const float4 *__restrict__ part,
@@ -1208,17 +1225,12 @@ __global__ __launch_bounds__(BLOCK) void distill_join(
     any = __ballot(any) != 0;
     wrong = __ballot(wrong) != 0;
     total = sum_wave_d(total);
-    double q_rest = 0., log_norm = 0., scale = 1., mass;
+    double q_rest = 0., mass = total;
     if (bucket) {
         q_rest = total < 1. ? 1. - total : 0.;
         mass = total + q_rest;
-    } else {
-        // not `total > 0`: NaN has to stay NaN
-        log_norm = total == 0. ? 0. : log_d(total);
-        scale = total == 0. ? 0. : 1. / total;
-        mass = total == 0. ? 0. : total / total;
     }
-    if (!any || (!bucket && total == 0.)) {
+    if (!any || (!bucket && total <= VOCAB_NO_MASS)) {
 #pragma unroll
         for (int e = 0; e < EPL; ++e)
             if (e * WAVE + lane < K)
@@ -1246,9 +1258,15 @@ __global__ __launch_bounds__(BLOCK) void distill_join(
             twice |= old != -1;
         }
     }
+    if (!bucket) {
+        mass = total / total;  // NaN stays NaN
+        const double scale = 1. / total;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) q[e] *= scale;
+    }
     double weight[EPL];
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) weight[e] = q[e] *= scale;
+    for (int e = 0; e < EPL; ++e) weight[e] = q[e];
     if (__ballot(twice)) {
         // rare: the first in order has the sum of all, in order
 #pragma unroll
@@ -1268,62 +1286,66 @@ __global__ __launch_bounds__(BLOCK) void distill_join(
             own[e] &= !before;
         }
     }
-#pragma unroll
-    for (int e = 0; e < EPL; ++e)
-        if (e * WAVE + lane < K)
-            entry[(long)r * K + e * WAVE + lane] =
-                make_int2(own[e] ? id[e] : -1,
-                          __float_as_int(own[e] ? (float)weight[e] : 0.f));
-
+    // with bucket, of the tokens that are not listed
     const RowStat st = join_parts(first_of, parts, g.nseg, c, lane);
-    double s = st.s;
+    double m = st.m, s = st.s, share = 1.;
     if (bucket) {
-        // the listed tokens' part, each token once
+        // and the listed ones, each once, against the largest of all
+        float high = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e)
+            if (own[e]) high = fmaxf(high, x[e]);
+        high = max_wave_f(high);
+        if (st.s == 0) m = high == -INFINITY ? 0. : high;
+        else m = fmax(m, (double)high);
+        share = exp2_d((st.m - m) * c);
         double s_in = 0.;
 #pragma unroll
         for (int e = 0; e < EPL; ++e)
-            if (own[e]) s_in += exp2_d(((double)x[e] - st.m) * c);
-        s += sum_wave_d(s_in);
+            if (own[e]) s_in += exp2_d((x[e] - m) * c);
+        s = sum_wave_d(s_in) + (st.s == 0 ? 0. : st.s * share);
     }
-    const bool none = s == 0, bad = !(s < INFINITY);
-    const double ln_s = log_d(s);
+    const bool none = s == 0, bad = !(s < INFINITY), nan = bad || wrong;
+    // entries that cover every token with mass leave no room for the rest;
+    // what 32-bit log probabilities leave over by rounding then counts as
+    // none
+    const double p_rest = bucket && !none && st.s != 0 ? st.s * share / s : 0.;
+    const bool open = q_rest > 0. && p_rest > VOCAB_NO_MASS;
+    const double ratio = open ? q_rest / p_rest : 1.;
+    const double ln_s = log_d(s), ln = log(bucket ? ratio : total);
+    const double scale = none ? 0. : mass / s;
     double sum = 0.;
 #pragma unroll
-    for (int e = 0; e < EPL; ++e)
-        if (id[e] >= 0 && q[e] != 0.) {
-            const double lp = none || x[e] == -INFINITY
-                                  ? -INFINITY
-                                  : ((double)x[e] - st.m) * inv_t - ln_s;
-            sum += q[e] * (((double)l[e] - log_norm) - lp);
-        }
-    sum = sum_wave_d(sum);
-    double ratio = 0.;
-    if (bucket && q_rest > 0.) {
-        // entries that cover every token with mass leave no room for
-        // the rest; what 32-bit log probabilities leave over by
-        // rounding then counts as none
-        const double p_rest = none ? 0. : st.s / s;
-        if (p_rest > 0.) {
-            ratio = q_rest / p_rest;
-            sum += q_rest * log(ratio);
-        } else if (q_rest > 0x1p-20) {
-            sum = INFINITY;
-        }
+    for (int e = 0; e < EPL; ++e) {
+        if (e * WAVE >= K) break;
+        const double lp = none || x[e] == -INFINITY
+                              ? -INFINITY : (x[e] - m) * inv_t - ln_s;
+        if (id[e] >= 0 && q[e] != 0.)
+            sum += q[e] * ((l[e] - (bucket ? 0. : ln)) - lp);
+        const double d = exp2_d((x[e] - m) * c) * scale;
+        if (e * WAVE + lane < K)
+            entry[(long)r * K + e * WAVE + lane] =
+                make_int2(own[e] ? id[e] : -1,
+                          __float_as_int(nan ? NAN : (float)(d - weight[e])));
     }
+    sum = sum_wave_d(sum);
+    if (open) sum += q_rest * ln;
+    else if (bucket && q_rest > 0x1p-20) sum = INFINITY;
     if (lane == 0) {
-        const bool nan = bad || wrong;
+        double a = mass * share / s;
+        if (open) a -= q_rest / st.s;
+        if (st.s == 0) a = 0.;
         loss[r] = nan ? NAN : (float)sum;
-        stat[r] = make_float4(st.m,
-                              none ? 0.f : (float)(exp2_d(-st.delta) / s),
-                              nan ? NAN : (float)mass,
-                              nan ? NAN : (float)(mass - ratio));
+        stat[r] = make_float4(st.m, nan ? NAN : (float)(a * exp2_d(-st.delta)),
+                              nan || !none ? 1.f : 0.f, 0.f);
     }
 }
 
 // ---- gradients -------------------------------------------------------------
-// d x_j = p_j (a + b ln(p_j s)) + what is given for single tokens, one wave per
-// stretch, in one pass over packed registers: a product, an exponential and
-// one or three more operations per element beside 4 or 8 bytes.
+// d x_j = p_j (a + b ln(p_j s)) + what is given for single tokens (in place of
+// it for a teacher's entries), one wave per stretch, in one pass over packed
+// registers: a product, an exponential and one or three more operations per
+// element beside 4 or 8 bytes.
 //
 // Single tokens (the given one, alternatives with a gradient, a teacher's
 // entries): those of the stretch are marked in LDS, a bit and a value each,
@@ -1362,8 +1384,7 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
     const long tok = !DISTILL && tokens ? tokens[r] : -1;
     const float g_row = d_row ? d_row[r] : 0.f;
     const float g_ent = !DISTILL && d_entropy ? d_entropy[r] : 0.f;
-    bool skip = st.y == 0.f;
-    if (DISTILL) skip = skip || (st.z == 0.f && st.w == 0.f);
+    bool skip = DISTILL ? st.z == 0.f : st.y == 0.f;
     if (!DISTILL && tokens && tok == ignore) skip = true;
     if (skip) {
         const float zero[N] = {};
@@ -1404,15 +1425,15 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
         const bool on = e * WAVE + lane < K;
         if (DISTILL) {
             id[e] = pair[e].x;
-            val[e] = -__int_as_float(pair[e].y);
+            val[e] = __int_as_float(pair[e].y);
         }
         const u64 off = id[e] - lo;
         at[e] = on && off < SEG && id[e] >= 0 ? (u32)off : SEG;
         if (!on) val[e] = 0.f;
     }
 
-    // e = 2^((x - m) c) counts k_out (k_in where listed) + k_d * exponent
-    float k_in = st.z, k_out = st.w, k_d = 0.f, scale = inv_t;
+    // e = 2^((x - m) c) counts k_out + k_d * exponent
+    float k_out = 1.f, k_d = 0.f, scale = inv_t;
     u32 tok_at = SEG;
     if (DISTILL) {
         scale *= g_row;
@@ -1431,7 +1452,7 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
             gs += sum_wave(gk);
         }
         k_d = -g_ent;
-        k_in = k_out = k_d * st.z - gs;
+        k_out = k_d * st.z - gs;
         k_d *= 0.69314718f;
     }
 
@@ -1463,7 +1484,7 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
     }
 
     const float mc = st.x * c, u = st.y * scale;
-    const float u_in = k_in * u, u_out = k_out * u, u_d = k_d * u;
+    const float u_out = k_out * u, u_d = k_d * u;
     auto one = [&](const Vec<T> &x, int j, auto diff) {
         float f[N];
         const bool listed = hit >> j & 1;
@@ -1472,19 +1493,16 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float d = diff(x.get(i));
-            float k = u_out;
-            if (DISTILL) {
-                if (listed && in >> i & 1) k = u_in;
-            } else {
-                // 2^-300 is 0, and (-inf) * 0 would be NaN
-                k = fmaf(u_d, fmaxf(d, -300.f), k);
-            }
+            // 2^-300 is 0, and (-inf) * 0 would be NaN
+            const float k =
+                DISTILL ? u_out : fmaf(u_d, fmaxf(d, -300.f), u_out);
             f[i] = exp2_hw(d) * k;
         }
         if (listed) {
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                f[i] += in >> i & 1 ? value[p + i] : 0.f;
+                if (in >> i & 1)
+                    f[i] = DISTILL ? value[p + i] : f[i] + value[p + i];
         }
         store_vec<STREAM_OUT>(orow, lo + p, g.V, f, whole);
     };

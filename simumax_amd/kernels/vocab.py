@@ -36,6 +36,7 @@ from . import insitu
 
 MAX_TOPK = 256       # VOCAB_MAX_K in csrc/vocab.h
 MAX_TOP_V = 524288   # VOCAB_MAX_TOP_V there
+NO_MASS = 1e-300     # VOCAB_NO_MASS in csrc/vocab.hip
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -64,8 +65,9 @@ def _check_logits(logits, temperature):
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits must be [..., V] with V >= 1, "
                          f"not {tuple(logits.shape)}")
-    if not (0.0 < float(temperature) < float("inf")):
-        raise ValueError(f"temperature must be positive and finite, "
+    # its reciprocal times log2(e) has to be a normal number of 32 bits
+    if not 1e-30 <= float(temperature) <= 1e30:
+        raise ValueError(f"temperature must be in [1e-30, 1e30], "
                          f"not {temperature}")
 
 
@@ -235,11 +237,12 @@ def _teacher_torch(teacher_logprobs, teacher_ids, V, bucket):
     if bucket:
         rest = torch.where(total < 1, 1 - total, 0.0)
     else:
-        q = torch.where(total == 0, 0.0, q / total)
-        l = l - torch.where(total == 0, 0.0, total.log())
+        vain = total <= NO_MASS
+        q = torch.where(vain, 0.0, q / total)
+        l = l - torch.where(vain, 0.0, total.log())
     left_out = ~held.any(-1, keepdim=True)
     if not bucket:
-        left_out = left_out | (total == 0)
+        left_out = left_out | vain
     return held, wrong, ids, l, q, rest, left_out
 
 
@@ -257,10 +260,11 @@ def _topk_distillation_torch(logits, teacher_logprobs, teacher_ids,
     ratio = torch.zeros_like(loss)
     if bucket:
         p_rest = torch.where(inside, 0.0, p).sum(-1, keepdim=True)
-        open_ = (q_rest > 0) & (p_rest > 0)
+        open_ = (q_rest > 0) & (p_rest > NO_MASS)
         ratio = torch.where(open_, q_rest / p_rest, 0.0)
         loss = loss + torch.where(open_, q_rest * ratio.log(), 0.0)
-        loss = torch.where((p_rest == 0) & (q_rest > 2.0 ** -20), inf, loss)
+        loss = torch.where((p_rest <= NO_MASS) & (q_rest > 2.0 ** -20), inf,
+                           loss)
     mass = q.sum(-1, keepdim=True) + q_rest
     d = p * torch.where(inside, mass, mass - ratio)
     d = d.scatter_add(-1, ids, -q)
@@ -317,16 +321,18 @@ def topk_distillation(logits, teacher_logprobs, teacher_ids, temperature=1.0,
     logits [..., V]; teacher_logprobs [..., K] at the same temperature, in
     any float type, and teacher_ids [..., K] int64, as ``token_logprobs``
     gives them (K <= 256); an id below 0 marks an absent entry, a row without
-    entries has loss 0 and no gradient. With l_k and i_k a row's entries and
-    p the student's probabilities:
+    entries has loss 0 and no gradient, as has one whose entries are to
+    be scaled and have a mass of no more than 1e-300. With l_k and i_k a row's
+    entries and p the student's probabilities:
 
     * ``tail="renormalize"``: the teacher's entries are scaled to sum to 1,
       q = softmax(l), and the loss is sum_k q_k (ln q_k - ln p[i_k]);
     * ``tail="bucket"``: q_k = exp(l_k), and what is left of the teacher,
       q_r = max(0, 1 - sum q), is compared with what the student gives to all
       tokens that are not listed, p_r: the loss gains q_r (ln q_r - ln p_r).
-      Where nothing is left of the student, q_r up to 2^-20 (the rounding of
-      32-bit log probabilities) counts as none, and more as +inf.
+      Where nothing is left of the student (p_r up to 1e-300), q_r up to 2^-20
+      (the rounding of 32-bit log probabilities) counts as none, and more as
+      +inf.
 
     Only the logits receive a gradient. The loss is not scaled by
     temperature^2."""

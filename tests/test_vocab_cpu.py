@@ -150,6 +150,35 @@ def edge_teachers(V, k, gen):
     return x, tlp, tid
 
 
+def far_teachers(V, k, gen, dtype=FP):
+    """Students that leave the tokens that are not listed less than 32 bits
+    hold, teachers whose entries have next to no mass."""
+    x = R.make_logits(8, V, FP, gen)
+    tlp, tid = R.make_teacher(x, k, 1.0, gen)
+    for r, gap in enumerate((95.0, 130.0, 500.0)):
+        x[r, tid[r]] += gap
+    x[3] -= 110.0                              # a mask of about -100
+    x[3, tid[3]] += 110.0
+    x[4, tid[4, 0]] += 200.0                   # one token has it all
+    tlp[5] -= 100.0
+    tlp[6] -= 600.0
+    tlp[7, 0] = -90.0
+    tid[7, 1:] = -1
+    return x.to(dtype), tlp, tid
+
+
+@pytest.mark.parametrize("tail", ["renormalize", "bucket"])
+def test_far_teachers(tail):
+    gen = _gen(6)
+    x, tlp, tid = far_teachers(123, 7, gen)
+    g = torch.randn(8, generator=gen)
+    xg = x.clone().requires_grad_(True)
+    loss = K.topk_distillation(xg, tlp, tid, tail=tail)
+    loss.backward(g)
+    R.check_distill(x, tlp, tid, 1.0, tail, loss, xg.grad, g)
+    assert loss.isfinite().all()
+
+
 @pytest.mark.parametrize("tail", ["renormalize", "bucket"])
 def test_edge_teachers(tail):
     gen = _gen(5)
@@ -274,6 +303,27 @@ def test_distillation_refuses(kw, err):
     args.update(kw)
     with pytest.raises(err):
         K.topk_distillation(**args)
+
+
+@pytest.mark.parametrize("T", [9e-31, 1.1e30, 1e-45, 1e300])
+def test_temperatures_past_32_bits_are_refused(T):
+    x = torch.zeros(2, 17)
+    ids = torch.zeros(2, 4, dtype=torch.int64)
+    with pytest.raises(ValueError):
+        K.token_logprobs(x, temperature=T)
+    with pytest.raises(ValueError):
+        K.topk_distillation(x, torch.zeros(2, 4), ids, temperature=T)
+
+
+@pytest.mark.parametrize("T", [1e-30, 1e30])
+def test_extreme_temperatures(T):
+    x = R.make_logits(4, 300, torch.float32, torch.Generator().manual_seed(5))
+    tok = torch.tensor([0, 1, int(x[2].argmax()), 299])
+    xg = x.clone().requires_grad_()
+    out = K.token_logprobs(xg, tok, topk=3, temperature=T)
+    g, h = torch.ones(4), torch.full((4,), 0.5)
+    torch.autograd.backward([out.logprobs, out.entropy], [g, h])
+    R.check_logprobs(x, tok, 3, T, out, (g, h, None), xg.grad)
 
 
 def test_limit_matches_the_kernels():

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 import vocab_reference as R
-from test_vocab_cpu import edge_logits, edge_teachers
+from test_vocab_cpu import edge_logits, edge_teachers, far_teachers
 
 pytestmark = pytest.mark.gpu
 
@@ -143,6 +143,22 @@ def test_huge_logits(dtype):
         R.check_logprobs(x, tok, 4, T, out, grads, d)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("T", [1e-30, 1e30])
+def test_extreme_temperatures(dtype, T):
+    V = 2500
+    x = R.make_logits(4, V, dtype, _gen(15))
+    tok = torch.tensor([0, 1, int(x[2].float().argmax()), V - 1])
+    grads = (torch.ones(4), torch.full((4,), 0.5), None)
+    out, d = run_logprobs(x, tok, 4, T, grads)
+    R.check_logprobs(x, tok, 4, T, out, grads, d)
+    tlp, tid = R.make_teacher(R.make_logits(4, V, dtype, _gen(16)), 6, 1.0,
+                              _gen(17))
+    for tail in ("renormalize", "bucket"):
+        loss, d = run_distill(x, tlp, tid, T, tail, grads[0])
+        R.check_distill(x, tlp, tid, T, tail, loss, d, grads[0])
+
+
 @pytest.mark.parametrize("tail", ["renormalize", "bucket"])
 @pytest.mark.parametrize("V", [123, 9001])
 def test_edge_teachers(tail, V):
@@ -152,6 +168,18 @@ def test_edge_teachers(tail, V):
     loss, d = run_distill(x, tlp, tid, 1.0, tail, g)
     R.check_distill(x, tlp, tid, 1.0, tail, loss, d, g)
     assert loss[0] == 0 and (d[0] == 0).all()
+
+
+@pytest.mark.parametrize("tail", ["renormalize", "bucket"])
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("V", [123, 9001])
+def test_far_teachers(tail, dtype, V):
+    gen = _gen(18)
+    x, tlp, tid = far_teachers(V, 7, gen, dtype)
+    g = torch.randn(8, generator=gen)
+    loss, d = run_distill(x, tlp, tid, 1.0, tail, g)
+    R.check_distill(x, tlp, tid, 1.0, tail, loss, d, g)
+    assert loss.isfinite().all()
 
 
 def test_teacher_in_one_place():

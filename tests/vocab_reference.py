@@ -139,9 +139,10 @@ def distill_row(x, teacher, temperature, tail, g=1.0):
         elif rest > 2.0 ** -20:
             loss = inf
     mass = sum(q) + rest
-    coef = torch.where(inside, mass, mass - ratio)
+    # of two Python numbers torch.where makes 32 bits
+    coef = mass - torch.where(inside, 0.0, ratio * torch.ones_like(p))
     grad = (p * coef - dense) * g / temperature
-    mag = p * torch.where(inside, mass, mass + ratio) + dense
+    mag = p * (2 * mass - coef) + dense
     err = (2 * 0.7 * (lp.clamp(min=-150).abs() / math.log(2)) + 20) * U \
         + 3 * SUM
     return (loss, bound + abs(loss) * 2 * U if loss < inf else 0.0, grad,
