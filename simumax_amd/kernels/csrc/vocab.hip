@@ -13,13 +13,19 @@
 // f_i with d_i = (m_i - m) c and f_i = 2^d_i.
 //
 // Three launches, none of which synchronises with the host:
-//   partials: one wave per 16-byte x 64 lanes x 8 stretch of a row, held in
+//   partials: one wave per stretch of 8 vectors of 16 bytes per lane, held in
 //             registers: one read for the maximum and the sums;
 //   join:     one wave per row (one workgroup where top alternatives are
-//             asked): statistics, loss;
-//   grad:     one wave per stretch again: p from the statistics, plus what
-//             the given tokens or the teacher's entries add.
+//             asked): statistics, loss, the teacher's entries' gradients;
+//   grad:     one wave per stretch of 4 vectors per lane: p from the
+//             statistics, and what is given for single tokens.
 // No floating-point atomics: the same input gives the same bits.
+//
+// A row is split over waves, not walked by one workgroup: 64 rows of 151936
+// fill the card as 8192 do, and no wave waits for another. What is measured
+// below are single launches back to back, of 8192 rows of 128257 bf16 where
+// no size is given. On the same card reading alone reaches 7.0-7.4 TB/s, and
+// copying 5.5-6.6 TB/s.
 #include <hip/hip_fp16.h>
 
 #include <type_traits>
@@ -224,8 +230,9 @@ template <typename T> DEV Vec<T> load_vec(const T *row, long at, long V) {
 
 // Stretches begin at a cache line (128 bytes) of what is streamed: the row's
 // first one lies up to a line before the row. Reads and, more so, writes of
-// whole lines are what the memory takes best: the gradient of 8192 rows of an
-// odd vocabulary of 128257 took 830 us, of 128384 tokens 698 us.
+// whole lines are what the memory takes best: with stretches that began at
+// the rows, the gradient of 8192 rows of 128257 bf16 took 830 us, and of 128384
+// tokens, whose rows all begin at a line, 698 us.
 DEV int before_row(const void *row, int size, u32 line) {
     return (int)((u32)(u64)row & line) / size;
 }
@@ -462,8 +469,12 @@ DEV u32 wave_index() {
 // With GRP also the maximum of each GROUP consecutive tokens, for the search
 // of the top alternatives.
 //
-// What bounds it: per element one unpacking, one product, one exponential,
-// one or two sums and half an operation for the maximum, beside 2 or 4 bytes.
+// What bounds it is the memory's read rate: 287 us (7.3 TB/s), 293 with the
+// entropy. Per element there are one unpacking, one product, one exponential,
+// one or two sums and half an operation for the maximum, beside 2 or 4 bytes;
+// the group maxima's exchange and their stores take it from 147 us to 162-187
+// at 4096 rows (145-150 without the stores). 512 rows of 102400 fp32 with
+// group maxima: 33 us (6.4 TB/s).
 template <typename T, bool ENT, bool EXCL, bool GRP, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void vocab_partials(
     VocabRows g, u32 first, const long *__restrict__ tokens, long ignore,
@@ -814,14 +825,17 @@ DEV bool bins_find(int K, int most, u32 top, u32 &bound, int &reach,
 // searched among the tokens themselves, and, where one value alone has too
 // many, a bound on the index. The whole takes NG maxima per thread.
 //
-// What bounds it is latency: barriers, and the groups' loads.
+// What bounds it is latency: barriers, and the groups' loads, of which
+// AHEAD vectors per thread are under way together. 4096 rows of 128257 with 64
+// alternatives 34-40 us (a search of the bound two bits at a time, without the
+// bins, and loads one by one: 94), one row 5.8 us, 512 rows of 102400 fp32 with
+// 128 alternatives 15.5 us.
 template <typename T, int NG>
 DEV void top_alternatives(const T *row, long g_V, int before, int G,
                           const u32 (&key)[NG], int K, TopShared &sh,
                           float *top_lp, long *top_ids) {
     constexpr int N = Vec<T>::N, LPG = GROUP / N;
-    // vectors per thread in flight
-    constexpr int AHEAD = 4;
+    constexpr int AHEAD = 4;  // 8 and 16 were no faster
     const int tid = threadIdx.x, lane = tid % WAVE, wid = tid / WAVE;
     int turn = 0;
     if (tid == 0) sh.n_group = sh.n_key = 0;
@@ -1090,7 +1104,8 @@ DEV RowOut logprobs_row(const RowIn<T> &in, const VocabRows &g,
     return o;
 }
 
-// without alternatives: one wave per row
+// without alternatives: one wave per row, 7.2 us for 8192 rows; a workgroup
+// per row, with its barriers, took 41
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void logprobs_join(
     VocabRows g, u32 first, const float4 *__restrict__ part,
@@ -1114,7 +1129,7 @@ __global__ __launch_bounds__(BLOCK) void logprobs_join(
                  tokens ? logprobs : nullptr, entropy, stat, lane);
 }
 
-// with alternatives: one workgroup per row
+// with alternatives: one workgroup per row, NG group maxima per thread
 template <typename T, int NG>
 __global__ __launch_bounds__(BLOCK) void logprobs_top_join(
     VocabRows g, u32 first, const float4 *__restrict__ part,
@@ -1185,6 +1200,9 @@ __global__ __launch_bounds__(BLOCK) void logprobs_top_join(
 // token's first. stat[r] = (m, a, live, 0), where the latter is a 2^(x*c - mc)
 // against the largest of the others: p_rest can be far below what 32 bits
 // hold. live is 0 where the row has no gradient.
+//
+// What bounds it is the latency of the entries' logits, which lie anywhere:
+// 8192 rows with 128 entries 30 us, 4096 with 64 entries 11 us.
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void distill_join(
     VocabRows g, u32 first, const float4 *__restrict__ part,
@@ -1355,8 +1373,12 @@ __global__ __launch_bounds__(BLOCK) void distill_join(
 // What bounds it is the memory, which takes reads and writes together best
 // from few waves with little each: the values' place in LDS (33 KB) leaves
 // four workgroups to a CU, and a stretch is half as long as in the forward
-// pass. Copying alone, 8192 rows of 128257 bf16: 765 us with 8 vectors per
-// lane and eight workgroups, 703 us with 4 and four.
+// pass. Copying alone took 765 us with 8 vectors per lane and eight
+// workgroups, 703 us with 4 and four, 669 us with rows at cache lines. The
+// gradient with a teacher's 128 entries takes 632 us (6.6 TB/s), of log
+// probabilities of a batch cut to its first S positions, half of whose rows
+// lie otherwise within their lines than the gradient's do, 735 us. Half the
+// workgroups again (960 us) and half the vectors (1137 us) were slower.
 template <typename T, bool DISTILL, bool STREAM_IN, bool STREAM_OUT>
 __global__ __launch_bounds__(BLOCK) void vocab_grad(
     VocabRows g, u32 nseg, u32 first, float c, float inv_t,

@@ -384,7 +384,8 @@ class LlamaForTraining(nn.Module):
 
     def logits(self, tokens):
         """[B, S] tokens -> [B, S, V] logits (the local sequence slice under
-        CP). A vocabulary sharded over tp has no whole rows to look at."""
+        CP), V with the padding that the training loss has too. A vocabulary
+        sharded over tp has no whole rows to look at."""
         if self.tp_size > 1:
             raise NotImplementedError(
                 "logits of a vocabulary sharded over tp are not gathered")
