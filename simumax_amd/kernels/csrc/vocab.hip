@@ -723,8 +723,8 @@ DEV int3 block_count(int a, int b, int c, TopShared &sh, int &turn) {
 
 // The largest bound, by `bits` bits from the top, that at least `least` keys
 // reach, two bits a turn; stops early where no more than `most` reach it.
-// counter(b) gives a wave's number of keys >= b. `reach` starts with how many
-// reach 0 and ends with how many reach the bound.
+// counter(a, b, c) gives a wave's numbers of keys >= a, >= b and >= c. `reach`
+// starts with how many reach 0 and ends with how many reach the bound.
 template <typename F>
 DEV u32 search_bound(int bits, int least, int most, int &reach, TopShared &sh,
                      int &turn, F counter) {
@@ -733,10 +733,9 @@ DEV u32 search_bound(int bits, int least, int most, int &reach, TopShared &sh,
     for (int shift = (bits - 1) & ~1; shift >= 0; shift -= 2) {
         // of an odd number of bits the first turn has only one
         const bool two = shift + 1 < bits;
-        const int a = counter(bound + (1u << shift));
-        const int b = two ? counter(bound + (2u << shift)) : 0;
-        const int c = two ? counter(bound + (3u << shift)) : 0;
-        const int3 n = block_count(a, b, c, sh, turn);
+        int3 n = counter(bound + (1u << shift), bound + (2u << shift),
+                         bound + (3u << shift));
+        n = block_count(n.x, two ? n.y : 0, two ? n.z : 0, sh, turn);
         const int step = n.z >= least ? 3 : n.y >= least ? 2
                          : n.x >= least                  ? 1 : 0;
         bound += (u32)step << shift;
@@ -848,11 +847,14 @@ DEV void top_alternatives(const T *row, long g_V, int before, int G,
         for (int i = 0; i < NG; ++i) bins_add<T>(key[i], top, sh);
         if (!bins_find<T>(K, most, top, bound, reach, sh))
             bound = search_bound(Order<T>::BITS, K, most, reach, sh, turn,
-                                 [&](u32 b) {
-                                     int n = 0;
+                                 [&](u32 a, u32 b, u32 c) {
+                                     int3 n = make_int3(0, 0, 0);
 #pragma unroll
-                                     for (int i = 0; i < NG; ++i)
-                                         n += __popcll(__ballot(key[i] >= b));
+                                     for (int i = 0; i < NG; ++i) {
+                                         n.x += __popcll(__ballot(key[i] >= a));
+                                         n.y += __popcll(__ballot(key[i] >= b));
+                                         n.z += __popcll(__ballot(key[i] >= c));
+                                     }
                                      return n;
                                  });
     }
@@ -982,19 +984,30 @@ DEV void top_alternatives(const T *row, long g_V, int before, int G,
     __syncthreads();
     int n = sh.n_key;
     if (n > CAP) {
-        auto count = [&](auto pred) {
-            int c = 0;
+        // the wave's numbers of tokens of which the three predicates hold
+        auto count = [&](auto a, auto b, auto c) {
+            int3 n = make_int3(0, 0, 0);
 #pragma unroll 1
             for (int i = 0; i < slots; i += BLOCK) {
                 const int at = where(i);
                 const Vec<T> x = vector(at);
 #pragma unroll
-                for (int k = 0; k < N; ++k)
-                    c += __popcll(
-                        __ballot(at + k >= 0 && at + k < V &&
-                                 pred(Order<T>::of(x.get(k)), (u32)at + k)));
+                for (int k = 0; k < N; ++k) {
+                    const bool in = at + k >= 0 && at + k < V;
+                    const u32 order = Order<T>::of(x.get(k));
+                    const u32 index = (u32)at + k;
+                    n.x += __popcll(__ballot(in && a(order, index)));
+                    n.y += __popcll(__ballot(in && b(order, index)));
+                    n.z += __popcll(__ballot(in && c(order, index)));
+                }
             }
-            return c;
+            return n;
+        };
+        auto never = [](u32, u32) { return false; };
+        auto count_above = [&]() {
+            const int3 c = count(
+                [&](u32 order, u32) { return order > bound; }, never, never);
+            return block_count(c.x, 0, 0, sh, turn).x;
         };
         // a count of the tokens themselves, as of the maxima before
         bins_clear<T, NG>(key, sh);
@@ -1007,24 +1020,52 @@ DEV void top_alternatives(const T *row, long g_V, int before, int G,
                 if (at + k >= 0 && at + k < V)
                     bins_add<T>(Order<T>::of(x.get(k)), top, sh);
         }
-        if (!bins_find<T>(K, CAP, top, bound, n, sh))
-            bound = search_bound(Order<T>::BITS, K, CAP, n, sh, turn, [&](u32 b) {
-                return count([&](u32 order, u32) { return order >= b; });
-            });
+        int above = -1;
+        if (!bins_find<T>(K, CAP, top, bound, n, sh)) {
+            // fewer than K above the bound: it is the K-th value itself, as
+            // where a mask leaves fewer than K tokens
+            above = count_above();
+            if (above < K)
+                n = CAP + 1;
+            else
+                bound = search_bound(
+                    Order<T>::BITS, K, CAP, n, sh, turn,
+                    [&](u32 a, u32 b, u32 c) {
+                        return count(
+                            [&](u32 order, u32) { return order >= a; },
+                            [&](u32 order, u32) { return order >= b; },
+                            [&](u32 order, u32) { return order >= c; });
+                    });
+        }
+        if (n > CAP && (above < 0 || above >= K)) above = count_above();
         if (n > CAP) {
-            // more than CAP tokens share the K-th value: `need` of them, the
-            // first ones
-            const int above =
-                count([&](u32 order, u32) { return order > bound; });
-            const int need = K - block_count(above, 0, 0, sh, turn).x;
-            index_bound = 0;
+            // more than CAP tokens with those that share the K-th value: of
+            // these the first ones, `need` or as many more as are ranked too.
+            // Two bits of the index a pass (3320 rows of 1570 fp32 of which
+            // 5 % are not masked, 128 alternatives: 82 us, one bit a pass and
+            // a search of the value before it 280)
+            const int need = K - above;
+            u32 from = 0;  // fewer than `need` come before it
 #pragma unroll 1
-            for (int bit = 30; bit >= 0; --bit) {
-                const u32 b = index_bound | 1u << bit;
-                const int c = count([&](u32 order, u32 index) {
-                    return order == bound && index < b;
-                });
-                if (block_count(c, 0, 0, sh, turn).x <= need) index_bound = b;
+            for (int shift = (31 - __clz(V)) & ~1; shift >= 0; shift -= 2) {
+                const u32 step = 1u << shift;
+                int3 c = count(
+                    [&](u32 order, u32 index) {
+                        return order == bound && index < from + step;
+                    },
+                    [&](u32 order, u32 index) {
+                        return order == bound && index < from + 2 * step;
+                    },
+                    [&](u32 order, u32 index) {
+                        return order == bound && index < from + 3 * step;
+                    });
+                c = block_count(c.x, c.y, c.z, sh, turn);
+                const int m = c.x >= need ? c.x : c.y >= need ? c.y : c.z;
+                const u32 steps = c.x >= need   ? 0
+                                  : c.y >= need ? 1 : c.z >= need ? 2 : 3;
+                from += steps * step;
+                index_bound = from + step;  // enough come before it
+                if (steps < 3 && above + m <= CAP) break;
             }
         }
         if (tid == 0) sh.n_key = 0;

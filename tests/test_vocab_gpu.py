@@ -591,6 +591,22 @@ def test_alternatives_of_few_groups(kind, dtype, V, topk):
     R.check_logprobs(x, None, topk, 1.0, out)
 
 
+@pytest.mark.parametrize("fill", [-math.inf, -1e4, 0.0])
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("V,topk", [(40000, 20), (40000, 256), (9001, 64)])
+def test_fewer_tokens_than_alternatives(fill, dtype, V, topk):
+    """A mask that leaves 0 to 300 tokens: what it fills is ranked by index."""
+    gen = _gen(97)
+    x = torch.full((5, V), fill)
+    for r, left in enumerate((0, 1, 3, 19, 300)):
+        at = torch.randperm(V, generator=gen)[:left]
+        x[r, at] = torch.rand(left, generator=gen) * 8 + 1
+    x[2, V - 1] = 0.5
+    x = x.to(dtype)
+    out = K.token_logprobs(x.to(DEV), topk=topk)
+    R.check_logprobs(x, None, topk, 1.0, out)
+
+
 def test_rows_of_every_alignment():
     """The same row at each of the 64 places within a cache line that a bf16
     row can begin at, read and written."""
