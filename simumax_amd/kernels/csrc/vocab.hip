@@ -228,11 +228,13 @@ template <typename T> DEV Vec<T> load_vec(const T *row, long at, long V) {
     return v;
 }
 
-// Stretches begin at a cache line (128 bytes) of what is streamed: the row's
-// first one lies up to a line before the row. Reads and, more so, writes of
-// whole lines are what the memory takes best: with stretches that began at
-// the rows, the gradient of 8192 rows of 128257 bf16 took 830 us, and of 128384
-// tokens, whose rows all begin at a line, 698 us.
+// Stretches begin at a cache line (128 bytes) of the logits: a row's first one
+// lies up to a line before the row. Whole lines are what the memory takes
+// best: with stretches that began at the rows, the gradient of 8192 rows of
+// 128257 bf16 took 830 us, and of 128384 tokens, whose rows all begin at a line,
+// 698 us. Where the gradient's rows lie otherwise in their lines than the
+// logits', it is the loads that gain by it: half of such rows 688 us, 738 with
+// stretches at lines of the gradient.
 DEV int before_row(const void *row, int size, u32 line) {
     return (int)((u32)(u64)row & line) / size;
 }
@@ -1418,7 +1420,7 @@ __global__ __launch_bounds__(BLOCK) void distill_join(
 // workgroups, 703 us with 4 and four, 669 us with rows at cache lines. The
 // gradient with a teacher's 128 entries takes 632 us (6.6 TB/s), of log
 // probabilities of a batch cut to its first S positions, half of whose rows
-// lie otherwise within their lines than the gradient's do, 735 us. Half the
+// lie otherwise within their lines than the gradient's do, 688 us. Half the
 // workgroups again (960 us) and half the vectors (1137 us) were slower.
 template <typename T, bool DISTILL, bool STREAM_IN, bool STREAM_OUT>
 __global__ __launch_bounds__(BLOCK) void vocab_grad(
@@ -1440,7 +1442,8 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
     if (w >= (u32)g.rows * nseg) return;
     const int r = w / nseg, seg = w - r * nseg;
     T *orow = out + (long)r * g.V;
-    const long lo = (long)seg * SEG - before_row(orow, sizeof(T), 127);
+    const T *row = row_ptr<T>(g, r);
+    const long lo = (long)seg * SEG - before_row(row, sizeof(T), 127);
     const bool whole = lo >= 0 && lo + SEG <= g.V;
     // the row's numbers come by scalar loads, which nothing queues behind
     const float4 st = stat[r];
@@ -1479,7 +1482,6 @@ __global__ __launch_bounds__(BLOCK) void vocab_grad(
             }
         }
     }
-    const T *row = row_ptr<T>(g, r);
     Vec<T> v[NGRAD];
     load_stretch<STREAM_IN>(row, lo, g.V, lane, v);
     u32 at[EPL];  // of the stretch, SEG or more where not in it
@@ -1692,9 +1694,10 @@ static void distill_fwd_t(const VocabRows &g, const VocabDistill &a,
 template <typename T>
 static void grad_t(const VocabRows &g, const VocabGrad &a, int distill,
                    void *out, hipStream_t stream) {
+    const long apart = g.stride_o | g.stride_i;  // its lowest bits are theirs
     const u32 nseg = (u32)vocab_stretches(
         g.V, sizeof(T), WAVE * NGRAD * Vec<T>::N,
-        (long)(u64)out % 128 || g.V * sizeof(T) % 128);
+        (long)(u64)g.base % 128 || apart * sizeof(T) % 128);
     const long bytes = logits_bytes(g, sizeof(T));
     auto kernel =
         bytes > STREAM_OUT_ABOVE ? (distill ? vocab_grad<T, true, true, true>
