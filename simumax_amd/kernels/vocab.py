@@ -47,10 +47,16 @@ class TokenLogprobs(NamedTuple):
     top_ids: Optional[torch.Tensor]       # [..., topk] int64
 
 
-def _hip(t):
-    from .ops import _use_hip, ext
+_ops = None  # imports this module: it is looked up at the first call
 
-    return ext() if _use_hip(t) else None
+
+def _hip(t):
+    global _ops
+    if not t.is_cuda:
+        return None
+    if _ops is None:
+        from . import ops as _ops
+    return _ops.ext()  # raises if missing
 
 
 def _record(name, nbytes):
@@ -62,19 +68,21 @@ def _check_logits(logits, temperature):
     if logits.dtype not in _DTYPES:
         raise TypeError(f"logits must be bf16, fp16 or fp32, "
                         f"not {logits.dtype}")
-    if logits.dim() < 1 or logits.shape[-1] < 1:
+    shape = logits.shape
+    if not shape or shape[-1] < 1:
         raise ValueError(f"logits must be [..., V] with V >= 1, "
-                         f"not {tuple(logits.shape)}")
+                         f"not {tuple(shape)}")
     # its reciprocal times log2(e) has to be a normal number of 32 bits
     if not 1e-30 <= float(temperature) <= 1e30:
         raise ValueError(f"temperature must be in [1e-30, 1e30], "
                          f"not {temperature}")
+    return shape
 
 
 def _check_ids(name, ids, shape, device):
     if ids.dtype != torch.int64:
         raise TypeError(f"{name} must be int64, not {ids.dtype}")
-    if tuple(ids.shape) != tuple(shape):
+    if ids.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)}, "
                          f"not {tuple(ids.shape)}")
     if ids.device != device:
@@ -203,8 +211,8 @@ def token_logprobs(logits, tokens=None, topk=0, temperature=1.0,
     Returns ``TokenLogprobs(logprobs, entropy, top_logprobs, top_ids)``, of
     which the first three are differentiable; what was not asked for is
     None."""
-    _check_logits(logits, temperature)
-    V = logits.shape[-1]
+    shape = _check_logits(logits, temperature)
+    V = shape[-1]
     if not 0 <= topk <= min(MAX_TOPK, V):
         raise ValueError(f"topk must be in [0, {min(MAX_TOPK, V)}] for a "
                          f"vocabulary of {V}, not {topk}")
@@ -212,7 +220,7 @@ def token_logprobs(logits, tokens=None, topk=0, temperature=1.0,
         raise ValueError(f"top alternatives of a vocabulary of {V}: at most "
                          f"{MAX_TOP_V}")
     if tokens is not None:
-        _check_ids("tokens", tokens, logits.shape[:-1], logits.device)
+        _check_ids("tokens", tokens, shape[:-1], logits.device)
         tokens = tokens.contiguous()
     args = (logits, tokens, int(topk), float(temperature), int(ignore_index))
     if logits.is_cuda and not insitu.ENABLED:
@@ -336,7 +344,7 @@ def topk_distillation(logits, teacher_logprobs, teacher_ids, temperature=1.0,
 
     Only the logits receive a gradient. The loss is not scaled by
     temperature^2."""
-    _check_logits(logits, temperature)
+    shape = _check_logits(logits, temperature)
     if tail not in ("renormalize", "bucket"):
         raise ValueError(f"tail must be 'renormalize' or 'bucket', "
                          f"not {tail!r}")
@@ -348,12 +356,12 @@ def topk_distillation(logits, teacher_logprobs, teacher_ids, temperature=1.0,
     if not 1 <= K <= MAX_TOPK:
         raise ValueError(f"a row takes 1 to {MAX_TOPK} teacher entries, "
                          f"not {K}")
-    shape = (*logits.shape[:-1], K)
+    shape = (*shape[:-1], K)
     _check_ids("teacher_ids", teacher_ids, shape, logits.device)
     if not teacher_logprobs.is_floating_point():
         raise TypeError(f"teacher_logprobs must be floating point, "
                         f"not {teacher_logprobs.dtype}")
-    if (tuple(teacher_logprobs.shape) != shape
+    if (teacher_logprobs.shape != shape
             or teacher_logprobs.device != logits.device):
         raise ValueError(f"teacher_logprobs must be {shape} on "
                          f"{logits.device}, not "
