@@ -412,6 +412,38 @@ def test_on_another_stream():
     R.check_distill(x, tlp, tid, 1.0, "bucket", loss, dd, g)
 
 
+def test_two_streams_at_once():
+    # calls in flight together share no workspace
+    k = 16
+    jobs = []
+    for i, (rows, V) in enumerate(((300, 32003), (40, 128257))):
+        gen = _gen(74 + i)
+        x = R.make_logits(rows, V, BF, gen)
+        tok = torch.randint(0, V, (rows,), generator=gen)
+        tlp, tid = R.make_teacher(x, k, 1.0, gen)
+        jobs.append([t.to(DEV) for t in (x, tok, tlp, tid)])
+
+    def work(x, tok, tlp, tid):
+        xg = x.detach().requires_grad_(True)
+        out = K.token_logprobs(xg, tok, topk=k)
+        loss = K.topk_distillation(xg, tlp, tid, tail="bucket")
+        d, = torch.autograd.grad(out.logprobs.sum() + loss.sum(), xg)
+        return [*out, loss, d]
+
+    want = [work(*j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = []
+    for _ in range(4):
+        for s, j in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                got.append(work(*j))
+    torch.cuda.synchronize()
+    for i, outs in enumerate(got):
+        for a, b in zip(outs, want[i % 2]):
+            assert torch.equal(a, b)
+
+
 def test_two_captured_graphs():
     """Forward and backward of both operators, captured into two graphs that
     are replayed in turn on new inputs, with eager calls in between."""
