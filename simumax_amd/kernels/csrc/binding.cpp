@@ -382,6 +382,10 @@ std::vector<torch::Tensor> token_logprobs_fwd(
     TORCH_CHECK(topk >= 0 && topk <= VOCAB_MAX_K && topk <= g.V, "topk");
     TORCH_CHECK(topk == 0 || g.V <= VOCAB_MAX_TOP_V,
                 "top alternatives of a vocabulary above ", VOCAB_MAX_TOP_V);
+    // what precedes a row in its first line is among its groups
+    TORCH_CHECK(topk == 0 || g.V + g.line / logits.element_size() <=
+                                 VOCAB_MAX_TOP_V,
+                "a row's groups are more than its threads hold");
     TORCH_CHECK(temperature > 0, "temperature");
     if (tokens) {
         CHECK_ROWS(*tokens, torch::kInt64, g.rows);

@@ -1616,7 +1616,7 @@ static long row_blocks(const VocabRows &g) {
     return CDIV((long)g.rows, (long)WAVES);
 }
 
-// stretches of a row; `shifted`: rows may begin within a line
+// stretches (or groups) of a row; `shifted`: rows may begin within a line
 static long vocab_stretches(long V, int size, int seg, bool shifted) {
     return CDIV(V + (shifted ? 127 / size : 0), (long)seg);
 }
@@ -1664,8 +1664,13 @@ static void logprobs_fwd_t(const VocabRows &g, const VocabLogprobs &a,
     }
     partials_t<T, true, false, true>(g, a.tokens, a.ignore, nullptr, 0, c,
                                      a.part, a.gmax, stream);
-    // maxima per thread; more than VOCAB_MAX_TOP_V tokens are refused before
-    const long per = CDIV(CDIV(g.V, (long)GROUP), (long)BLOCK);
+    // maxima per thread, of a row that begins as late within a line as rows
+    // can (the kernel counts groups from the line, as stretches are counted):
+    // rows of 65535 bf16 have 1024 groups or 1025. More than VOCAB_MAX_TOP_V
+    // are refused before
+    const long groups =
+        vocab_stretches(g.V, sizeof(T), GROUP, g.line != 0);
+    const long per = CDIV(groups, (long)BLOCK);
     if (per <= 4) logprobs_top_join_t<T, 4>(g, a, c, stream);
     else if (per <= 8) logprobs_top_join_t<T, 8>(g, a, c, stream);
     else if (per <= 16) logprobs_top_join_t<T, 16>(g, a, c, stream);

@@ -665,3 +665,28 @@ def test_rows_of_every_alignment():
         R.check_logprobs(cpu, tok, k, 1.0, out, (one, one, None), d1)
         R.check_distill(cpu, tlp.expand(64, k), tid.expand(64, k), 1.0,
                         "bucket", loss, d2, one)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("V,wider", [
+    (65529, 0), (65535, 0), (131071, 0), (262143, 0),
+    # whole numbers of groups per thread, in rows off the cache lines
+    (65536, 3), (131072, 8), (262144, 5),
+    # the last vocabulary whose stretches begin at lines, and the next one
+    (524160, 0), (524161, 0)])
+def test_alternatives_at_the_end(V, wider, dtype):
+    """The largest tokens are a row's last ones, in rows that begin anywhere
+    within a cache line: the groups of 64 are one more than V has."""
+    gen = _gen(V + wider)
+    rows = 3
+    wide = R.make_logits(rows, V + wider, dtype, gen)
+    x = wide[..., :V]
+    x[:, V - 40:] = (20 + 5 * torch.rand(rows, 40, generator=gen)).to(dtype)
+    x[2, :V - 30] = -math.inf  # nothing but the end is left
+    xg = wide.to(DEV)[..., :V].detach().requires_grad_(True)
+    for topk in (1, 20, 256):
+        print("topk", topk, flush=True)
+        gk = torch.randn(rows, topk, generator=gen)
+        out = K.token_logprobs(xg, topk=topk)
+        d, = torch.autograd.grad(out.top_logprobs, xg, gk.to(DEV))
+        R.check_logprobs(x, None, topk, 1.0, out, (None, None, gk), d)
