@@ -1273,7 +1273,8 @@ __global__ __launch_bounds__(BLOCK) void distill_join(
         l[e] = k < K ? tlp[(long)r * K + k] : 0.f;
         any |= i >= 0;
         wrong |= i >= g.V;
-        id[e] = i < g.V ? (int)i : -1;
+        // (the low half of an id below -2^31 can be any number)
+        id[e] = i >= 0 && i < g.V ? (int)i : -1;
         if (i < 0) l[e] = -INFINITY;
     }
 #pragma unroll

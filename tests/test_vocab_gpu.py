@@ -690,3 +690,23 @@ def test_alternatives_at_the_end(V, wider, dtype):
         out = K.token_logprobs(xg, topk=topk)
         d, = torch.autograd.grad(out.top_logprobs, xg, gk.to(DEV))
         R.check_logprobs(x, None, topk, 1.0, out, (None, None, gk), d)
+
+
+@pytest.mark.parametrize("tail", ["renormalize", "bucket"])
+def test_entries_marked_absent_by_any_number_below_zero(tail):
+    # numbers whose low 32 bits are a token, or lie far outside the row
+    gen = _gen(101)
+    V, k = 9001, 8
+    x = R.make_logits(4, V, BF, gen)
+    tlp, tid = R.make_teacher(x, k, 1.0, gen)
+    tid[0, 2:7] = torch.tensor([-2 ** 63, -2 ** 32, -2 ** 32 + 5,
+                                -2 ** 31 - 1, -2 ** 31])
+    tid[1, 0] = -2 ** 32 + int(tid[1, 1])   # a token that is listed, too
+    tid[2] = -2 ** 31 - 1 - torch.arange(k)
+    tid[3, 1:] = -2 ** 40 + torch.arange(1, k)
+    g = torch.randn(4, generator=gen)
+    loss, d = run_distill(x, tlp, tid, 1.0, tail, g)
+    R.check_distill(x, tlp, tid, 1.0, tail, loss, d, g)
+    assert loss[2] == 0 and (d[2] == 0).all()
+    same, d2 = run_distill(x, tlp, tid.clamp(min=-1), 1.0, tail, g)
+    assert torch.equal(loss, same) and torch.equal(d, d2)
