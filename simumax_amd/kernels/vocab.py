@@ -255,8 +255,8 @@ def _teacher_torch(teacher_logprobs, teacher_ids, V, bucket):
 
 
 def _topk_distillation_torch(logits, teacher_logprobs, teacher_ids,
-                             temperature, bucket):
-    """Losses, and each row's gradient for a loss that counts 1."""
+                             temperature, bucket, dloss=None):
+    """Losses, or, given theirs, the logits' gradients."""
     V = logits.shape[-1]
     z, s, p, none, bad = _softmax_torch(logits, temperature)
     held, wrong, ids, l, q, q_rest, left_out = _teacher_torch(
@@ -273,15 +273,18 @@ def _topk_distillation_torch(logits, teacher_logprobs, teacher_ids,
         loss = loss + torch.where(open_, q_rest * ratio.log(), 0.0)
         loss = torch.where((p_rest <= NO_MASS) & (q_rest > 2.0 ** -20), inf,
                            loss)
+    nan = bad | wrong
+    if dloss is None:
+        loss = torch.where(nan, float("nan"), loss)
+        return torch.where(left_out, 0.0, loss).squeeze(-1).float()
     mass = q.sum(-1, keepdim=True) + q_rest
     d = p * torch.where(inside, mass, mass - ratio)
     d = d.scatter_add(-1, ids, -q)
-    d = torch.where(none, 0.0, d / temperature)
-    nan = bad | wrong
-    loss = torch.where(nan, float("nan"), loss)
+    # the rows without a gradient last: they have none of a NaN either
+    d = d * dloss.double()[..., None] / temperature
+    d = torch.where(none, 0.0, d)
     d = torch.where(nan, float("nan"), d)
-    loss = torch.where(left_out, 0.0, loss).squeeze(-1)
-    return loss.float(), torch.where(left_out, 0.0, d)
+    return torch.where(left_out, 0.0, d).to(logits.dtype)
 
 
 class _TopkDistillationFn(torch.autograd.Function):
@@ -291,7 +294,7 @@ class _TopkDistillationFn(torch.autograd.Function):
         ctx.args = (temperature, bucket)
         e = _hip(logits)
         if e is None:
-            loss, _ = _topk_distillation_torch(
+            loss = _topk_distillation_torch(
                 logits, teacher_logprobs, teacher_ids, temperature, bucket)
             ctx.save_for_backward(logits, teacher_logprobs, teacher_ids, None)
             return loss
@@ -309,10 +312,9 @@ class _TopkDistillationFn(torch.autograd.Function):
         logits, teacher, entry, stat = ctx.saved_tensors
         temperature, bucket = ctx.args
         if stat is None:
-            _, d = _topk_distillation_torch(logits, teacher, entry,
-                                            temperature, bucket)
-            d = (d * dloss.double()[..., None]).to(logits.dtype)
-            return d, None, None, None, None
+            return _topk_distillation_torch(
+                logits, teacher, entry, temperature, bucket,
+                dloss), None, None, None, None
         stop = _record("bw_topk_distillation_bwd",
                        2 * logits.numel() * logits.element_size())
         d = _hip(logits).topk_distillation_bwd(dloss.contiguous(), logits,

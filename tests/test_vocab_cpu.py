@@ -334,3 +334,37 @@ def test_limit_matches_the_kernels():
     with open(path) as f:
         assert int(re.search(r"VOCAB_MAX_K (\d+)", f.read()).group(1)) \
             == VO.MAX_TOPK
+
+
+def check_rows_without_a_gradient(device):
+    """Left-out rows and rows without a finite logit have a gradient of zero,
+    whatever comes from above for them."""
+    gen = _gen(13)
+    V, k = 300, 5
+    x = R.make_logits(5, V, FP, gen)
+    x[1] = -math.inf
+    tlp, tid = R.make_teacher(R.make_logits(5, V, FP, gen), k, 1.0, gen)
+    tid[0] = -1
+    tlp[2] = -math.inf          # nothing to scale to 1
+    tok = torch.tensor([-100, 3, -100, 4, 5])
+    x, tlp, tid, tok = (t.to(device) for t in (x, tlp, tid, tok))
+    for bad in (math.nan, math.inf):
+        g = torch.tensor([bad, bad, bad, 1.0, bad], device=device)
+        for tail, zero in (("renormalize", (0, 1, 2)), ("bucket", (0, 1))):
+            xg = x.clone().requires_grad_(True)
+            loss = K.topk_distillation(xg, tlp, tid, tail=tail)
+            loss.backward(g)
+            for r in zero:
+                assert (xg.grad[r] == 0).all(), (tail, bad, r)
+            assert xg.grad[3].isfinite().all()
+            assert not xg.grad[4].isfinite().any()
+        xg = x.clone().requires_grad_(True)
+        out = K.token_logprobs(xg, tok, topk=2)
+        torch.autograd.backward((out.logprobs, out.entropy), (g, g))
+        for r in (0, 1, 2):
+            assert (xg.grad[r] == 0).all(), (bad, r)
+        assert xg.grad[3].isfinite().all()
+
+
+def test_rows_without_a_gradient():
+    check_rows_without_a_gradient("cpu")

@@ -7,7 +7,8 @@ import math
 import pytest
 import torch
 import vocab_reference as R
-from test_vocab_cpu import edge_logits, edge_teachers, far_teachers
+from test_vocab_cpu import (check_rows_without_a_gradient, edge_logits,
+                            edge_teachers, far_teachers)
 
 pytestmark = pytest.mark.gpu
 
@@ -710,3 +711,7 @@ def test_entries_marked_absent_by_any_number_below_zero(tail):
     assert loss[2] == 0 and (d[2] == 0).all()
     same, d2 = run_distill(x, tlp, tid.clamp(min=-1), 1.0, tail, g)
     assert torch.equal(loss, same) and torch.equal(d, d2)
+
+
+def test_rows_without_a_gradient():
+    check_rows_without_a_gradient(DEV)
