@@ -17,6 +17,7 @@ import torch.utils.cpp_extension as cpp_ext
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "simumax_hip.so")
+FLAGS = os.path.join(HERE, "simumax_hip.flags")  # what OUT was built with
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
 
 KERNEL_SOURCES = ["rmsnorm.hip", "rope.hip", "swiglu.hip", "cross_entropy.hip", "fp8_cast.hip",
@@ -29,15 +30,19 @@ def _newest_mtime(paths):
     return max(os.path.getmtime(p) for p in paths if os.path.exists(p))
 
 
+def _recorded_flags():
+    if not os.path.exists(FLAGS):
+        return None
+    with open(FLAGS) as f:
+        return f.read()
+
+
 def build(verbose: bool = True, force: bool = False) -> str:
     sources = [os.path.join(CSRC, s) for s in KERNEL_SOURCES
                if os.path.exists(os.path.join(CSRC, s))]
     sources.append(os.path.join(CSRC, "wgrad.cpp"))
     sources.append(os.path.join(CSRC, "binding.cpp"))
     headers = [os.path.join(CSRC, h) for h in HEADERS]
-    if (not force and os.path.exists(OUT)
-            and os.path.getmtime(OUT) > _newest_mtime(sources + headers)):
-        return OUT
 
     inc = [f"-I{p}" for p in cpp_ext.include_paths()]
     inc.append(f"-I{sysconfig.get_paths()['include']}")
@@ -57,6 +62,21 @@ def build(verbose: bool = True, force: bool = False) -> str:
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     ]
 
+    link_flags = [
+        f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10",
+        "-lc10_hip", "-ltorch_python", "-lhipblas", f"-Wl,-rpath,{torch_lib}",
+    ]
+
+    # objects of other flags are no newer for being newer than their source
+    flags = "\n".join(common + inc + link_flags)
+    if _recorded_flags() != flags:
+        force = True
+        if os.path.exists(FLAGS):
+            os.remove(FLAGS)
+    if (not force and os.path.exists(OUT)
+            and os.path.getmtime(OUT) > _newest_mtime(sources + headers)):
+        return OUT
+
     def compile_one(src):
         obj = os.path.join(HERE, os.path.basename(src) + ".o")
         if (not force and os.path.exists(obj)
@@ -73,13 +93,12 @@ def build(verbose: bool = True, force: bool = False) -> str:
     with ThreadPoolExecutor(max_workers=8) as pool:
         objs = list(pool.map(compile_one, sources))
 
-    link = ["hipcc", "-shared", "-o", OUT] + objs + [
-        f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10",
-        "-lc10_hip", "-ltorch_python", "-lhipblas", f"-Wl,-rpath,{torch_lib}",
-    ]
+    link = ["hipcc", "-shared", "-o", OUT] + objs + link_flags
     if verbose:
         print("[simumax_hip] linking", OUT)
     subprocess.run(link, check=True)
+    with open(FLAGS, "w") as f:
+        f.write(flags)
     return OUT
 
 
