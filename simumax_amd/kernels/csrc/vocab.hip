@@ -570,15 +570,19 @@ __global__ __launch_bounds__(BLOCK) void vocab_partials(
     const float m = from_pattern<T>(m_bits);
     const float mr = m == -INFINITY ? 0.f : m, mc = mr * c;
     float s = 0.f, t = 0.f;
-    // one vector; the values stay packed until here
+    // one vector; the values stay packed until here. Summed by itself first:
+    // beside a lane's token that has nearly all of a row, 7 terms each lose
+    // what 32 bits lack, not 63
     auto sums = [&](const Vec<T> &x, auto diff) {
+        float sv;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float d = diff(x.get(i)), e = exp2_hw(d);
-            s += e;
+            sv = i == 0 ? e : sv + e;
             // 2^-300 is 0, and (-inf) * 0 would be NaN; NaN is in e already
             if (ENT) t = fmaf(fmaxf(d, -300.f), e, t);
         }
+        s += sv;
     };
     if (by_product(mc)) {
 #pragma unroll

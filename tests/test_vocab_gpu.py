@@ -715,3 +715,25 @@ def test_entries_marked_absent_by_any_number_below_zero(tail):
 
 def test_rows_without_a_gradient():
     check_rows_without_a_gradient(DEV)
+
+
+@pytest.mark.parametrize("dtype,V", [(BF, 4096), (HF, 4096), (FP, 2048)])
+def test_many_small_terms_beside_a_large_one(dtype, V):
+    """One token has all of a row but V terms of e^-17, each below half a step
+    of 1 in 32 bits: a sum in order would lose every one of its lane's."""
+    x = torch.full((3, V), -17.0, dtype=dtype)
+    tok = torch.tensor([0, V // 2 + 5, V - 1])
+    x[torch.arange(3), tok] = 0.0
+    want = torch.full((3,), -math.log1p((V - 1) * math.exp(-17.0)),
+                      dtype=torch.float64)
+    # of one vector at most N - 1 terms, 0.7 u each, then a rounding for each
+    # of the lane's other 7 vectors and of the wave's 6 additions, beside which
+    # the terms' own errors (of V e^-17 < 2e-4) are below 1 u
+    N = 4 if dtype == FP else 8
+    bound = (0.7 * (N - 1) + 7 + 6 + 1) * R.U
+    assert 0.7 * (8 * N - 1) * R.U > bound   # what a sum in order loses
+    out = K.token_logprobs(x.to(DEV), tok.to(DEV))
+    R.assert_close(out.logprobs, want, bound, "logprobs")
+    loss = K.topk_distillation(x.to(DEV), torch.zeros(3, 1, device=DEV),
+                               tok[:, None].to(DEV))
+    R.assert_close(loss, -want, bound, "loss")
