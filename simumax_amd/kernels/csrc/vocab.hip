@@ -103,10 +103,6 @@ typedef __hip_bfloat16 bf16;
 DEV float to_f(float v) { return v; }
 DEV float to_f(__half v) { return __half2float(v); }
 DEV float to_f(bf16 v) { return __bfloat162float(v); }
-template <typename T> DEV T from_f(float v);
-template <> DEV float from_f<float>(float v) { return v; }
-template <> DEV __half from_f<__half>(float v) { return __float2half(v); }
-template <> DEV bf16 from_f<bf16>(float v) { return __float2bfloat16(v); }
 
 template <> DEV float Vec<float>::get(int i) const {
     return __uint_as_float(w[i]);
