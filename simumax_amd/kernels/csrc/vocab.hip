@@ -467,12 +467,13 @@ DEV u32 wave_index() {
 // With GRP also the maximum of each GROUP consecutive tokens, for the search
 // of the top alternatives.
 //
-// What bounds it is the memory's read rate: 287 us (7.3 TB/s), 293 with the
-// entropy. Per element there are one unpacking, one product, one exponential,
-// one or two sums and half an operation for the maximum, beside 2 or 4 bytes;
-// the group maxima's exchange and their stores take it from 147 us to 162-187
-// at 4096 rows (145-150 without the stores). 512 rows of 102400 fp32 with
-// group maxima: 33 us (6.4 TB/s).
+// What bounds it is the memory's read rate: 288-292 us (shortest and median
+// launch; 7.2-7.3 TB/s), 294-309 with the entropy. Per element there are one
+// unpacking, one product, one exponential, one or two sums and half an
+// operation for the maximum, beside 2 or 4 bytes: the vector units issue in a
+// fifth of the cycles. The group maxima's exchange and their stores take it
+// from 147 us to 162-190 at 4096 rows (145-150 without the stores). 512 rows of
+// 102400 fp32 with group maxima: 33-34 us (6.2-6.4 TB/s).
 template <typename T, bool ENT, bool EXCL, bool GRP, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void vocab_partials(
     VocabRows g, u32 first, const long *__restrict__ tokens, long ignore,
@@ -827,10 +828,10 @@ DEV bool bins_find(int K, int most, u32 top, u32 &bound, int &reach,
 // many, a bound on the index. The whole takes NG maxima per thread.
 //
 // What bounds it is latency: barriers, and the groups' loads, of which
-// AHEAD vectors per thread are under way together. 4096 rows of 128257 with 64
-// alternatives 34-40 us (a search of the bound two bits at a time, without the
-// bins, and loads one by one: 94), one row 5.8 us, 512 rows of 102400 fp32 with
-// 128 alternatives 15.5 us.
+// AHEAD vectors per thread are under way together (waves wait in 61 % of their
+// cycles). 4096 rows of 128257 with 64 alternatives 34-41 us (a search of the
+// bound two bits at a time, without the bins, and loads one by one: 94), one
+// row 6 us, 512 rows of 102400 fp32 with 128 alternatives 15-16 us.
 template <typename T, int NG>
 DEV void top_alternatives(const T *row, long g_V, int before, int G,
                           const u32 (&key)[NG], int K, TopShared &sh,
@@ -1147,7 +1148,7 @@ DEV RowOut logprobs_row(const RowIn<T> &in, const VocabRows &g,
     return o;
 }
 
-// without alternatives: one wave per row, 7.2 us for 8192 rows; a workgroup
+// without alternatives: one wave per row, 7-8 us for 8192 rows; a workgroup
 // per row, with its barriers, took 41
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void logprobs_join(
@@ -1244,8 +1245,9 @@ __global__ __launch_bounds__(BLOCK) void logprobs_top_join(
 // against the largest of the others: p_rest can be far below what 32 bits
 // hold. live is 0 where the row has no gradient.
 //
-// What bounds it is the latency of the entries' logits, which lie anywhere:
-// 8192 rows with 128 entries 30 us, 4096 with 64 entries 11 us.
+// What bounds it is the latency of the entries' logits, which lie anywhere
+// (waves wait in 71 % of their cycles): 8192 rows with 128 entries 30-31 us, 4096
+// with 64 entries 12 us.
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void distill_join(
     VocabRows g, u32 first, const float4 *__restrict__ part,
@@ -1419,9 +1421,9 @@ __global__ __launch_bounds__(BLOCK) void distill_join(
 // four workgroups to a CU, and a stretch is half as long as in the forward
 // pass. Copying alone took 765 us with 8 vectors per lane and eight
 // workgroups, 703 us with 4 and four, 669 us with rows at cache lines. The
-// gradient with a teacher's 128 entries takes 632 us (6.6 TB/s), of log
+// gradient with a teacher's 128 entries takes 632-649 us (6.5-6.6 TB/s), of log
 // probabilities of a batch cut to its first S positions, half of whose rows
-// lie otherwise within their lines than the gradient's do, 688 us. Half the
+// lie otherwise within their lines than the gradient's do, 689-695 us. Half the
 // workgroups again (960 us) and half the vectors (1137 us) were slower.
 template <typename T, bool DISTILL, bool STREAM_IN, bool STREAM_OUT>
 __global__ __launch_bounds__(BLOCK) void vocab_grad(

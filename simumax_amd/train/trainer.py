@@ -510,7 +510,10 @@ def distill_step(model, teacher, opt, reducer, tokens, micro_batch_num=1,
     """``train_step`` from a teacher: per microbatch the teacher's pass gives
     its topk log probabilities, and the student takes the gradient of its
     divergence from them. Teacher and student share tokens and vocabulary;
-    neither's is sharded (tp = 1)."""
+    neither's is sharded (tp = 1). As in ``train_step`` every position counts;
+    prompts and padding are left out by ``distillation_loss`` with teacher ids
+    of -1, as the teacher's ``token_logprobs`` gives them where a target is
+    ``ignore_index``."""
     opt.zero_grad()
     total_loss = 0.0
     for mb in range(micro_batch_num):
